@@ -41,6 +41,15 @@ extern "C" {
 #define RKV_BF16 1
 #define RKV_I8 2  /* int8 bytes + one fp32 scale per (token, KV head) row   */
 #define RKV_FP8 3 /* OCP fp8 e4m3 bytes + one fp32 scale per row            */
+#define RKV_I8_BLOCK 4  /* int8 bytes + one fp32 scale per (block, KV head)     */
+#define RKV_FP8_BLOCK 5 /* e4m3 bytes + one power of two per (block, KV head)   */
+
+/* Frequency scalings of rkv_rope_frequencies. */
+#define RKV_ROPE_PLAIN 0
+#define RKV_ROPE_LINEAR 1
+#define RKV_ROPE_BASE 2
+#define RKV_ROPE_PARTS 3
+#define RKV_ROPE_BANDS 4
 
 #define RKV_OK 0
 #define RKV_ERR_INVALID_ARG (-1) /* maps to CoreError::InvalidArgument / Shape */
@@ -318,6 +327,188 @@ int rkv_prefill_attention(float* out, const float* q, const void* k_pool, const 
                           int num_q_heads, int num_kv_heads, int head_dim, int block_size,
                           int64_t num_blocks, int max_q_len, float scale, int dtype,
                           void* stream);
+
+/* ---- rotary positions ---------------------------------------------------------
+ * No counterpart in the reference, whose positions are the sinusoids added to
+ * the embedding (crates/nn/src/transformer.rs:69-82); decoders with grouped KV
+ * heads rotate q and k between the projections and the cache instead.
+ *
+ * Pair i < rotary_dim / 2 of a row at position p turns by the angle
+ * p * inv_freq[i] (radians), formed in 64 bits:
+ *   y0 = magnitude (x0 cos - x1 sin),  y1 = magnitude (x1 cos + x0 sin)
+ * with (x0, x1) the elements (i, i + rotary_dim / 2), or with interleaved != 0
+ * (2 i, 2 i + 1).  Elements from rotary_dim on pass unchanged.  positions:
+ * int32 [n_tokens], any value (the negative position turns back).  inv_freq:
+ * double [rotary_dim / 2] on the device (rkv_rope_frequencies). */
+
+/* Rotates rows x[t][h] of head_dim fp32 elements into out.  Strides in
+ * elements, multiples of 4; pointers 16-byte aligned; out may be x with the
+ * same strides, else they must not overlap.  head_dim a multiple of 8 up to
+ * 1024, rotary_dim even and <= head_dim. */
+int rkv_rope(float* out, const float* x, const int32_t* positions, const double* inv_freq,
+             int64_t n_tokens, int num_heads, int head_dim, int rotary_dim,
+             int64_t out_tok_stride, int64_t out_head_stride, int64_t tok_stride,
+             int64_t head_stride, int interleaved, float magnitude, void* stream);
+
+/* One layer's rotation and KV append in one launch: q rows [n_tokens][Hq] are
+ * rotated into q_out, k_new rows [n_tokens][Hkv] are rotated and appended,
+ * v_new rows are appended, at slot_mapping[t] (a slot that rkv_append skips is
+ * skipped here; its q rows are rotated all the same).  q_out and the pools
+ * equal rkv_rope of q and of k_new followed by rkv_append (RKV_F32, RKV_BF16)
+ * or rkv_append_q (RKV_I8, RKV_FP8, whose scale pools are k_scale / v_scale;
+ * NULL for the others), bit for bit.  k_new and v_new share src_tok_stride and
+ * src_head_stride.  Block-scaled pools: rkv_rope, then rkv_append_block_q. */
+int rkv_rope_append(float* q_out, void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                    const float* q, const float* k_new, const float* v_new,
+                    int64_t out_tok_stride, int64_t out_head_stride, int64_t q_tok_stride,
+                    int64_t q_head_stride, int64_t src_tok_stride, int64_t src_head_stride,
+                    const int32_t* positions, const double* inv_freq,
+                    const int64_t* slot_mapping, int64_t n_tokens, int num_q_heads,
+                    int num_kv_heads, int head_dim, int rotary_dim, int interleaved,
+                    float magnitude, int block_size, int64_t num_blocks, int dtype,
+                    void* stream);
+
+/* The frequency table of a rotary configuration (host memory): inv_freq
+ * [rotary_dim / 2] and the magnitude to pass with it.  f_i = base^(-2 i /
+ * rotary_dim), then by scaling:
+ *   RKV_ROPE_PLAIN   f_i
+ *   RKV_ROPE_LINEAR  f_i / factor (position interpolation)
+ *   RKV_ROPE_BASE    f_i of base * factor^(rotary_dim / (rotary_dim - 2))
+ *   RKV_ROPE_PARTS   between f_i / factor and f_i by a ramp over the pairs from
+ *                    the one that turns `high` times within original_context
+ *                    (rounded down) to the one that turns `low` times (rounded
+ *                    up); magnitude 0.1 ln(factor) + 1 (the YaRN method; low 1
+ *                    and high 32 are its usual values)
+ *   RKV_ROPE_BANDS   f_i for pairs that turn `high` times or more within
+ *                    original_context, f_i / factor for those under `low`,
+ *                    linear in the number of turns between
+ * magnitude is 1 elsewhere.  base > 1; factor >= 1 (unused by PLAIN);
+ * original_context > 0 and 0 < low < high for PARTS and BANDS. */
+int rkv_rope_frequencies(double* inv_freq, float* magnitude, int rotary_dim, double base,
+                         int scaling, double factor, int64_t original_context, double low,
+                         double high);
+
+/* ---- 8-bit pools with a scale for each block and KV head -----------------------
+ * Byte pools laid out like the row-scaled ones, scale pools [num_blocks][Hkv]
+ * fp32: 1/16 of the row-scaled formats' scale bytes, and one scale for the
+ * whole (block, head) tile an attention kernel reads.  value = byte * scale.
+ *   RKV_I8_BLOCK:  the scale is max |x| over the tile's rows times 1 / 127 (both
+ *                  rounded to fp32), byte = x / scale rounded to nearest even.
+ *   RKV_FP8_BLOCK: the scale is the smallest power of two s with max |x| / s <=
+ *                  448, byte = e4m3 of x / s, rounded to nearest even: a larger
+ *                  scale later leaves earlier rows' bytes exact (but for those
+ *                  that become subnormal).
+ * Rows are rounded once per growth of their block's scale: when rows join a
+ * block, scale' = max(scale, the new rows' own) and, where it grew, the older
+ * rows' bytes become byte * scale / scale' rounded the same way.  A growth
+ * costs an int8 row at most half a step of the new scale.  Only finite values
+ * count for a scale: an infinity becomes the largest magnitude, a NaN is 0 in
+ * RKV_I8_BLOCK and NaN in RKV_FP8_BLOCK.  A tile whose largest magnitude is
+ * below 2^-110 is stored as zeros with scale 0.
+ * rkv_gather_q, rkv_decode_attention_q take these dtypes with their scale pools.
+ * Compaction: rkv_copy_blocks on the byte pools, and on the scale pools with
+ * block_bytes = Hkv * 4 where that is a multiple of 16 (else the caller moves
+ * the scales). */
+
+/* Append into block-scaled pools, every layer in one launch.  Sequence b's new
+ * rows are rows new_start[b] .. new_start[b+1]-1 of k_new / v_new; ctx_lens[b]
+ * counts them already: the n_b rows belong at positions ctx_lens[b] - n_b ..
+ * ctx_lens[b] - 1 of block_tables[b] (int32 [num_seqs][max_blocks_per_seq]).
+ * All rows of a call that fall in a block are quantized together with the rows
+ * that stand before them in it; a block whose first row is new takes no regard
+ * of what its memory held.  max_new: host-side bound on the n_b (it sizes the
+ * grid); only the first max_new rows of a sequence are written.  Negative
+ * positions, positions past the table and block ids outside the pool are
+ * skipped.  A block must not be appended to through two sequences of the call.
+ * Strides as rkv_append; pool_layer_stride in bytes, the scale pools' is
+ * pool_layer_stride / (16 * head_dim).  block_size 16; head_dim 32, 64 or 128. */
+int rkv_append_block_q(void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                       int64_t pool_layer_stride, const float* k_new, const float* v_new,
+                       int64_t src_layer_stride, int64_t src_tok_stride,
+                       int64_t src_head_stride, const int32_t* new_start,
+                       const int32_t* block_tables, int max_blocks_per_seq,
+                       const int32_t* ctx_lens, int num_seqs, int n_layers, int num_kv_heads,
+                       int head_dim, int block_size, int64_t num_blocks, int max_new, int dtype,
+                       void* stream);
+
+/* rkv_prefill_attention over block-scaled pools (RKV_I8_BLOCK, RKV_FP8_BLOCK;
+ * row-scaled pools are RKV_ERR_UNSUPPORTED): the same result as prefill on the
+ * dequantized values.  head_dim 64 or 128. */
+int rkv_prefill_attention_q(float* out, const float* q, const void* k_pool, const void* v_pool,
+                            const float* k_scale, const float* v_scale,
+                            const int32_t* block_tables, int max_blocks_per_seq,
+                            const int32_t* q_start, const int32_t* ctx_lens, int num_seqs,
+                            int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                            int64_t num_blocks, int max_q_len, float scale, int dtype,
+                            void* stream);
+
+/* ---- eviction by accumulated attention weight -----------------------------------
+ * No counterpart in the reference, which evicts whole requests
+ * (crates/nn/src/continuous_batching.rs:380-386).  A weight pool holds one fp32
+ * sum per cached row, [num_blocks][Hkv][block_size]: decode steps add the
+ * softmax weights each row received, and a sequence that outgrows its share
+ * keeps, per KV head, the rows of the largest sums beside its first and its
+ * latest ones.  The caller clears a block's sums when it hands the block to a
+ * sequence. */
+
+/* Workspace (bytes) of rkv_decode_attention_weights: the split-K partials and
+ * the scores of up to max_context tokens a sequence. */
+size_t rkv_decode_weights_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int max_context);
+
+/* rkv_decode_attention (any dtype; k_scale / v_scale are the scale pools of the
+ * 1-byte formats, else NULL) that also adds to weights[block][kv head][row] the
+ * softmax weight the row received, summed over the KV head's query heads.  A
+ * row of a block that stands in several of the call's tables (a shared prefix)
+ * receives every one's weight, in no fixed order; other rows' sums do not
+ * depend on the order of anything.  Rows past a context and blocks with an
+ * invalid id receive nothing. */
+int rkv_decode_attention_weights(float* out, float* weights, const float* q, const void* k_pool,
+                                 const void* v_pool, const float* k_scale, const float* v_scale,
+                                 const int32_t* block_tables, int max_blocks_per_seq,
+                                 const int32_t* ctx_lens, int num_seqs, int num_q_heads,
+                                 int num_kv_heads, int head_dim, int block_size,
+                                 int64_t num_blocks, int max_context, float scale, int dtype,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which rows each (layer, sequence, KV head) keeps: of the L_b = ctx_lens[b]
+ * positions (clamped to max_blocks_per_seq * block_size) whose block id is
+ * valid, all if they are at most budget, else budget of them: positions below
+ * `sinks` and the last `recent` before L_b first, then the largest weights (a
+ * tie goes to the lower position, a NaN ranks below every number).
+ *   keep      int32 [n_layers][num_seqs][Hkv][budget]: kept positions in
+ *             ascending order, then -1
+ *   new_lens  int32 [num_seqs]: how many were kept (the same in every layer
+ *             and KV head)
+ * Layer l's sums start at weights + l * weights_layer_stride (elements).
+ * budget > 0, sinks, recent >= 0, sinks + recent <= budget; max_context: as
+ * rkv_decode_attention (positions from it on are treated as past L_b);
+ * block_size 16. */
+int rkv_evict_select(int32_t* keep, int32_t* new_lens, const float* weights,
+                     int64_t weights_layer_stride, const int32_t* block_tables,
+                     int max_blocks_per_seq, const int32_t* ctx_lens, int num_seqs,
+                     int n_layers, int num_kv_heads, int block_size, int64_t num_blocks,
+                     int budget, int sinks, int recent, int max_context, void* stream);
+
+/* Moves the kept rows of every (layer, sequence, KV head) to positions 0 ..
+ * new_lens[b] - 1 of dst_tables[b], in every layer's K and V pool, scale pools
+ * (NULL without) and weight pool (NULL: left alone).  No destination block may
+ * stand in a source table of the call or twice among the destinations; the
+ * source blocks are left as they are (other sequences may share them) for the
+ * caller to free.  Kept positions past the source table and rows of invalid
+ * blocks are skipped, rows from new_lens[b] on are left as they were.
+ * Block-scaled pools: a destination tile takes the largest scale of its rows'
+ * tiles, and bytes are rounded to it as in rkv_append_block_q.
+ * pool_layer_stride in elements of the pools, as rkv_append / rkv_append_q;
+ * keep, new_lens and budget as rkv_evict_select; head_dim a multiple of 8 (1-byte
+ * pools: 32, 64 or 128); block_size 16. */
+int rkv_evict_compact(void* k_pool, void* v_pool, float* k_scale, float* v_scale, float* weights,
+                      int64_t pool_layer_stride, int64_t weights_layer_stride,
+                      const int32_t* keep, const int32_t* new_lens, int budget,
+                      const int32_t* src_tables, int src_blocks_per_seq,
+                      const int32_t* dst_tables, int dst_blocks_per_seq, int num_seqs,
+                      int n_layers, int num_kv_heads, int head_dim, int block_size,
+                      int64_t num_blocks, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -104,6 +104,39 @@ int rkv_transpose(float* y, const float* x, int m, int n, void* stream);
  * element i unless the current best is greater. */
 int rkv_argmax(int32_t* out, const float* x, int rows, int n, void* stream);
 
+/* Workspace (bytes) of rkv_process_logits with a pick. */
+size_t rkv_process_logits_workspace_bytes(int rows, int n);
+
+/* Penalties, biases and masks on logits, and the greedy pick, for requests that
+ * Sampler::greedy (crates/nn/src/continuous_batching.rs:458-462) alone does not
+ * serve; no counterpart in the reference.  Row r of logits [rows][n] (row_stride
+ * elements apart) becomes row r of out ([rows][n], out_stride apart; out may be
+ * logits with the same stride):
+ *   1. tokens of the row's history: x > 0 ? x / repetition[r] : x * repetition[r]
+ *   2. x -= frequency[r] * count + presence[r], for tokens with count > 0, the
+ *      number of times the token stands in the history from prompt_lens[r] on
+ *   3. x += the token's bias (the last of the row's entries for it)
+ *   4. tokens whose bit in the row's mask is 0 become -infinity
+ * history: int32 token ids, row r's are history[history_start[r] ..
+ * history_start[r+1]-1] (history_start: int32 [rows + 1]); the first
+ * prompt_lens[r] of them are the prompt.  repetition, frequency, presence: fp32
+ * [rows].  bias_ids / bias with bias_start [rows + 1] likewise.  allowed:
+ * 32-bit words [rows][allowed_stride], token c is bit c % 32 of word c / 32.
+ * pick: int32 [rows], rkv_argmax's rule on the result with a NaN taken as
+ * -infinity (the last index among equal maxima), and -1 where every entry is
+ * -infinity.  Ids outside [0, n) are skipped.
+ * Any of repetition, frequency, presence, prompt_lens (no prompt), bias_ids,
+ * allowed and pick may be NULL, history too when none of the first three is
+ * given; with out NULL only the pick is made.  The workspace is needed for a
+ * pick.  rows <= 65535. */
+int rkv_process_logits(float* out, int64_t out_stride, int32_t* pick, const float* logits,
+                       int64_t row_stride, int rows, int n, const int32_t* history,
+                       const int32_t* history_start, const int32_t* prompt_lens,
+                       const float* repetition, const float* frequency, const float* presence,
+                       const int32_t* bias_ids, const float* bias, const int32_t* bias_start,
+                       const int32_t* allowed, int64_t allowed_stride, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* ---- greedy decoder (benchmark configs[0]) ------------------------------------
  * Pre-LN causal decoder: x = E[id] + PE[pos]; per layer h = LN1(x),
  * q,k,v = h W^T + b, K/V appended to a paged fp32 pool (16-token blocks from

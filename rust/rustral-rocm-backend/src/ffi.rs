@@ -16,6 +16,14 @@ pub const RKV_F32: c_int = 0;
 pub const RKV_BF16: c_int = 1;
 pub const RKV_I8: c_int = 2;
 pub const RKV_FP8: c_int = 3;
+pub const RKV_I8_BLOCK: c_int = 4;
+pub const RKV_FP8_BLOCK: c_int = 5;
+
+pub const RKV_ROPE_PLAIN: c_int = 0;
+pub const RKV_ROPE_LINEAR: c_int = 1;
+pub const RKV_ROPE_BASE: c_int = 2;
+pub const RKV_ROPE_PARTS: c_int = 3;
+pub const RKV_ROPE_BANDS: c_int = 4;
 
 pub const RKV_OK: c_int = 0;
 pub const RKV_ERR_INVALID_ARG: c_int = -1;
@@ -365,6 +373,194 @@ extern "C" {
         dtype: c_int,
         stream: Stream,
     ) -> c_int;
+
+    pub fn rkv_rope(
+        out: *mut f32,
+        x: *const f32,
+        positions: *const i32,
+        inv_freq: *const f64,
+        n_tokens: i64,
+        num_heads: c_int,
+        head_dim: c_int,
+        rotary_dim: c_int,
+        out_tok_stride: i64,
+        out_head_stride: i64,
+        tok_stride: i64,
+        head_stride: i64,
+        interleaved: c_int,
+        magnitude: f32,
+        stream: Stream,
+    ) -> c_int;
+
+    pub fn rkv_rope_append(
+        q_out: *mut f32,
+        k_pool: *mut c_void,
+        v_pool: *mut c_void,
+        k_scale: *mut f32,
+        v_scale: *mut f32,
+        q: *const f32,
+        k_new: *const f32,
+        v_new: *const f32,
+        out_tok_stride: i64,
+        out_head_stride: i64,
+        q_tok_stride: i64,
+        q_head_stride: i64,
+        src_tok_stride: i64,
+        src_head_stride: i64,
+        positions: *const i32,
+        inv_freq: *const f64,
+        slot_mapping: *const i64,
+        n_tokens: i64,
+        num_q_heads: c_int,
+        num_kv_heads: c_int,
+        head_dim: c_int,
+        rotary_dim: c_int,
+        interleaved: c_int,
+        magnitude: f32,
+        block_size: c_int,
+        num_blocks: i64,
+        dtype: c_int,
+        stream: Stream,
+    ) -> c_int;
+
+    pub fn rkv_rope_frequencies(
+        inv_freq: *mut f64,
+        magnitude: *mut f32,
+        rotary_dim: c_int,
+        base: f64,
+        scaling: c_int,
+        factor: f64,
+        original_context: i64,
+        low: f64,
+        high: f64,
+    ) -> c_int;
+
+    pub fn rkv_append_block_q(
+        k_pool: *mut c_void,
+        v_pool: *mut c_void,
+        k_scale: *mut f32,
+        v_scale: *mut f32,
+        pool_layer_stride: i64,
+        k_new: *const f32,
+        v_new: *const f32,
+        src_layer_stride: i64,
+        src_tok_stride: i64,
+        src_head_stride: i64,
+        new_start: *const i32,
+        block_tables: *const i32,
+        max_blocks_per_seq: c_int,
+        ctx_lens: *const i32,
+        num_seqs: c_int,
+        n_layers: c_int,
+        num_kv_heads: c_int,
+        head_dim: c_int,
+        block_size: c_int,
+        num_blocks: i64,
+        max_new: c_int,
+        dtype: c_int,
+        stream: Stream,
+    ) -> c_int;
+
+    pub fn rkv_prefill_attention_q(
+        out: *mut f32,
+        q: *const f32,
+        k_pool: *const c_void,
+        v_pool: *const c_void,
+        k_scale: *const f32,
+        v_scale: *const f32,
+        block_tables: *const i32,
+        max_blocks_per_seq: c_int,
+        q_start: *const i32,
+        ctx_lens: *const i32,
+        num_seqs: c_int,
+        num_q_heads: c_int,
+        num_kv_heads: c_int,
+        head_dim: c_int,
+        block_size: c_int,
+        num_blocks: i64,
+        max_q_len: c_int,
+        scale: f32,
+        dtype: c_int,
+        stream: Stream,
+    ) -> c_int;
+
+    pub fn rkv_decode_weights_workspace_bytes(
+        num_seqs: c_int,
+        num_q_heads: c_int,
+        num_kv_heads: c_int,
+        head_dim: c_int,
+        max_context: c_int,
+    ) -> usize;
+
+    pub fn rkv_decode_attention_weights(
+        out: *mut f32,
+        weights: *mut f32,
+        q: *const f32,
+        k_pool: *const c_void,
+        v_pool: *const c_void,
+        k_scale: *const f32,
+        v_scale: *const f32,
+        block_tables: *const i32,
+        max_blocks_per_seq: c_int,
+        ctx_lens: *const i32,
+        num_seqs: c_int,
+        num_q_heads: c_int,
+        num_kv_heads: c_int,
+        head_dim: c_int,
+        block_size: c_int,
+        num_blocks: i64,
+        max_context: c_int,
+        scale: f32,
+        dtype: c_int,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: Stream,
+    ) -> c_int;
+
+    pub fn rkv_evict_select(
+        keep: *mut i32,
+        new_lens: *mut i32,
+        weights: *const f32,
+        weights_layer_stride: i64,
+        block_tables: *const i32,
+        max_blocks_per_seq: c_int,
+        ctx_lens: *const i32,
+        num_seqs: c_int,
+        n_layers: c_int,
+        num_kv_heads: c_int,
+        block_size: c_int,
+        num_blocks: i64,
+        budget: c_int,
+        sinks: c_int,
+        recent: c_int,
+        max_context: c_int,
+        stream: Stream,
+    ) -> c_int;
+
+    pub fn rkv_evict_compact(
+        k_pool: *mut c_void,
+        v_pool: *mut c_void,
+        k_scale: *mut f32,
+        v_scale: *mut f32,
+        weights: *mut f32,
+        pool_layer_stride: i64,
+        weights_layer_stride: i64,
+        keep: *const i32,
+        new_lens: *const i32,
+        budget: c_int,
+        src_tables: *const i32,
+        src_blocks_per_seq: c_int,
+        dst_tables: *const i32,
+        dst_blocks_per_seq: c_int,
+        num_seqs: c_int,
+        n_layers: c_int,
+        num_kv_heads: c_int,
+        head_dim: c_int,
+        block_size: c_int,
+        num_blocks: i64,
+        dtype: c_int,
+        stream: Stream,
+    ) -> c_int;
     // ---- include/rustral_model.h
     pub fn rkv_embed(
         out: *mut f32,
@@ -431,6 +627,35 @@ extern "C" {
         -> c_int;
     pub fn rkv_transpose(y: *mut f32, x: *const f32, m: c_int, n: c_int, stream: Stream) -> c_int;
     pub fn rkv_argmax(out: *mut i32, x: *const f32, rows: c_int, n: c_int, stream: Stream) -> c_int;
+
+    pub fn rkv_process_logits_workspace_bytes(
+        rows: c_int,
+        n: c_int,
+    ) -> usize;
+
+    pub fn rkv_process_logits(
+        out: *mut f32,
+        out_stride: i64,
+        pick: *mut i32,
+        logits: *const f32,
+        row_stride: i64,
+        rows: c_int,
+        n: c_int,
+        history: *const i32,
+        history_start: *const i32,
+        prompt_lens: *const i32,
+        repetition: *const f32,
+        frequency: *const f32,
+        presence: *const f32,
+        bias_ids: *const i32,
+        bias: *const f32,
+        bias_start: *const i32,
+        allowed: *const i32,
+        allowed_stride: i64,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: Stream,
+    ) -> c_int;
     pub fn rkv_decoder_param_count(cfg: *const RkvDecoderConfig) -> i64;
     pub fn rkv_decoder_init_params(
         cfg: *const RkvDecoderConfig,

@@ -11,12 +11,15 @@ import os
 from .build import LIB_PATH
 
 RKV_F32, RKV_BF16, RKV_I8, RKV_FP8 = 0, 1, 2, 3
+RKV_I8_BLOCK, RKV_FP8_BLOCK = 4, 5
+RKV_ROPE_PLAIN, RKV_ROPE_LINEAR, RKV_ROPE_BASE, RKV_ROPE_PARTS, RKV_ROPE_BANDS = 0, 1, 2, 3, 4
 RKV_OK = 0
 RKV_ERR_INVALID_ARG, RKV_ERR_UNSUPPORTED, RKV_ERR_WORKSPACE, RKV_ERR_HIP = -1, -2, -3, -4
 RKV_ERR_OOM = -5
 
 # Every symbol include/rustral_kv.h declares, with (restype, argtypes).
 _p, _i, _i64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
+_d = C.c_double
 SIGNATURES = {
     "rkv_last_error": (C.c_char_p, []),
     "rkv_version": (_i, []),
@@ -47,6 +50,21 @@ SIGNATURES = {
                                     _i, _f, _i, _i, _p, _sz, _p]),
     "rkv_decode_attention_append_q": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i,
                                            _i, _i, _i, _i64, _i, _f, _i, _i, _p, _sz, _p]),
+    "rkv_rope": (_i, [_p, _p, _p, _p, _i64, _i, _i, _i, _i64, _i64, _i64, _i64, _i, _f, _p]),
+    "rkv_rope_append": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+                             _p, _p, _p, _i64, _i, _i, _i, _i, _i, _f, _i, _i64, _i, _p]),
+    "rkv_rope_frequencies": (_i, [_p, _p, _i, _d, _i, _d, _i64, _d, _d]),
+    "rkv_append_block_q": (_i, [_p, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i, _p,
+                                _i, _i, _i, _i, _i, _i64, _i, _i, _p]),
+    "rkv_prefill_attention_q": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i,
+                                     _i64, _i, _f, _i, _p]),
+    "rkv_decode_weights_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "rkv_decode_attention_weights": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i,
+                                          _i, _i64, _i, _f, _i, _p, _sz, _p]),
+    "rkv_evict_select": (_i, [_p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i64, _i, _i, _i, _i,
+                              _p]),
+    "rkv_evict_compact": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _i, _p, _i, _p, _i, _i, _i,
+                               _i, _i, _i, _i64, _i, _p]),
     # include/rustral_serving.h (host memory)
     "rkv_dbm_create": (_p, [_i64, _i, _i, _i, _p]),
     "rkv_dbm_destroy": (None, [_p]),
@@ -94,6 +112,9 @@ SIGNATURES = {
     "rkv_matmul": (_i, [_p, _p, _p, _i, _i, _i, _p]),
     "rkv_transpose": (_i, [_p, _p, _i, _i, _p]),
     "rkv_argmax": (_i, [_p, _p, _i, _i, _p]),
+    "rkv_process_logits_workspace_bytes": (_sz, [_i, _i]),
+    "rkv_process_logits": (_i, [_p, _i64, _p, _p, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                                _p, _i64, _p, _sz, _p]),
     "rkv_decoder_param_count": (_i64, [_p]),
     "rkv_decoder_init_params": (_i, [_p, C.c_uint64, _f, _p]),
     "rkv_decoder_create": (_p, [_p, _p, _i64, _p]),

@@ -4,8 +4,8 @@
 
 namespace rkv {
 
-Launch decode_bf16(int D, int G, int P, bool append) {
-  return pick_d<uint16_t, RKV_BF16>(D, G, P, append);
+Launch decode_bf16(int D, int G, int P, DecodeMode mode) {
+  return pick_d<uint16_t, RKV_BF16>(D, G, P, mode);
 }
 
 }  // namespace rkv

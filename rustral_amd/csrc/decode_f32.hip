@@ -3,8 +3,8 @@
 
 namespace rkv {
 
-Launch decode_f32(int D, int G, int P, bool append) {
-  return pick_d<float, RKV_F32>(D, G, P, append);
+Launch decode_f32(int D, int G, int P, DecodeMode mode) {
+  return pick_d<float, RKV_F32>(D, G, P, mode);
 }
 
 }  // namespace rkv

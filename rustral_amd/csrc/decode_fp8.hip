@@ -3,8 +3,8 @@
 
 namespace rkv {
 
-Launch decode_fp8(int D, int G, int P, bool append) {
-  return pick_d<uint8_t, RKV_FP8>(D, G, P, append);
+Launch decode_fp8(int D, int G, int P, DecodeMode mode) {
+  return pick_d<uint8_t, RKV_FP8>(D, G, P, mode);
 }
 
 }  // namespace rkv

@@ -4,8 +4,8 @@
 
 namespace rkv {
 
-Launch decode_i8(int D, int G, int P, bool append) {
-  return pick_d<uint8_t, RKV_I8>(D, G, P, append);
+Launch decode_i8(int D, int G, int P, DecodeMode mode) {
+  return pick_d<uint8_t, RKV_I8>(D, G, P, mode);
 }
 
 }  // namespace rkv

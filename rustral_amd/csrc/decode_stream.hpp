@@ -1,6 +1,7 @@
 // decode_stream.hpp -- the split-K decode kernel of paged_decode.hip and the
 // choice of its build, compiled once per pool format (decode_f32.hip,
-// decode_bf16.hip, decode_i8.hip, decode_fp8.hip).
+// decode_bf16.hip, decode_i8.hip, decode_fp8.hip, and for the formats with one
+// scale a tile decode_i8_block.hip, decode_fp8_block.hip).
 //
 // Pass 1 (decode_stream_kernel) splits every sequence into partitions of P
 // tokens and produces, per (partition, query head), the partial softmax state
@@ -44,15 +45,22 @@ struct Launch {
   int nw = 0;
   void (*kernel)(float*, float*, float*, const float*, const void*, const void*, const float*,
                  const float*, const int32_t*, int, const int32_t*, int, int, int64_t, float,
-                 int, int, const float*, const float*) = nullptr;
+                 int, int, const float*, const float*, float*) = nullptr;
 };
+
+// What a build does beside the attention: nothing, the append of the step's new
+// row (fused), or leaving every score and every partition's (m, l) behind for
+// the pass that adds up the rows' weights.
+enum DecodeMode { kAttend, kAppend, kScores };
 
 // The build for head_dim D, G query heads per KV head and partitions of P
 // tokens; a null kernel where there is none.
-Launch decode_f32(int D, int G, int P, bool append);
-Launch decode_bf16(int D, int G, int P, bool append);
-Launch decode_i8(int D, int G, int P, bool append);
-Launch decode_fp8(int D, int G, int P, bool append);
+Launch decode_f32(int D, int G, int P, DecodeMode mode);
+Launch decode_bf16(int D, int G, int P, DecodeMode mode);
+Launch decode_i8(int D, int G, int P, DecodeMode mode);
+Launch decode_fp8(int D, int G, int P, DecodeMode mode);
+Launch decode_i8_block(int D, int G, int P, DecodeMode mode);
+Launch decode_fp8_block(int D, int G, int P, DecodeMode mode);
 
 namespace {
 
@@ -289,8 +297,14 @@ __device__ __forceinline__ float lo_col(float x) {
 // rkv_append does) into the pools before it streams its tiles, and reads
 // them back with the rest of the tile.  Nothing else in the launch reads
 // the row.
-template <typename T, int D, int G, int BS, int NTILE, int R, int SPLIT, int FMT,
-          bool APPEND = false>
+// kScores: scores (fp32 [num_seqs][Hkv][score_stride][G], score_stride =
+// max_parts P) receives the log2-domain scores of every position below the
+// context, -inf where the block id is invalid, and part_ml every partition's
+// (m, l), also a sequence's only one.
+// Formats with one scale a tile (RKV_I8_BLOCK, RKV_FP8_BLOCK) run the row-scaled
+// formats' code with the tile's scale in the place of its rows'.
+template <typename T, int D, int G, int BS, int NTILE, int R, int SPLIT, int FORMAT,
+          DecodeMode MODE = kAttend>
 __global__ __launch_bounds__(64 * SPLIT)
 __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) void decode_stream_kernel(
     float* __restrict__ out, float* __restrict__ part_acc, float* __restrict__ part_ml,
@@ -299,7 +313,11 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
     const float* __restrict__ v_scale, const int32_t* __restrict__ block_tables,
     int max_blocks_per_seq, const int32_t* __restrict__ ctx_lens, int ctx_cap, int num_kv_heads,
     int64_t num_blocks, float q_scale, int max_parts, int tiles_per_wave,
-    const float* __restrict__ k_new, const float* __restrict__ v_new) {
+    const float* __restrict__ k_new, const float* __restrict__ v_new,
+    float* __restrict__ scores) {
+  constexpr bool APPEND = MODE == kAppend;
+  constexpr bool TSC = FORMAT == RKV_I8_BLOCK || FORMAT == RKV_FP8_BLOCK;
+  constexpr int FMT = FORMAT == RKV_I8_BLOCK ? RKV_I8 : FORMAT == RKV_FP8_BLOCK ? RKV_FP8 : FORMAT;
   const T* __restrict__ k_pool = static_cast<const T*>(k_pool_);
   const T* __restrict__ v_pool = static_cast<const T*>(v_pool_);
   constexpr int E = Traits<T>::E;
@@ -590,14 +608,17 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
   };
   if constexpr (QNT) {
 #pragma unroll
-    for (int i = 0; i < NTW; ++i) ksc[i] = ld_scale(k_scale + base[i] / D + kt);
+    for (int i = 0; i < NTW; ++i)
+      ksc[i] = TSC ? k_scale[base[i] / (BS * D)] : ld_scale(k_scale + base[i] / D + kt);
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
       const int x = lane + 64 * j, ix = x / BS;
       int64_t rb = base[0];  // base[ix] by selects (ix differs between lanes)
 #pragma unroll
       for (int i = 1; i < NTW; ++i) rb = ix == i ? base[i] : rb;
-      vsc[j] = x < NTW * BS ? ld_scale(v_scale + rb / D + x % BS) : 0.0f;
+      vsc[j] = x >= NTW * BS ? 0.0f
+               : TSC         ? v_scale[rb / (BS * D)]
+                             : ld_scale(v_scale + rb / D + x % BS);
     }
   }
 
@@ -805,6 +826,25 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // LDS writes above ...
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");  // ... before the reads below
+        if constexpr (MODE == kScores) {
+          // this slice's scores, G to a position: contiguous over the wave
+          float* sp = scores + (((int64_t)b * num_kv_heads + kh) * ((int64_t)max_parts * P) + tok0) * G;
+          const int live = tw * BS < L - tok0 ? tw * BS : L - tok0;  // may be <= 0
+#pragma unroll
+          for (int x = lane; x < NTW * BS; x += 64)
+            if (x < live) {
+              if constexpr (G % 4 == 0) {
+#pragma unroll
+                for (int g = 0; g < G; g += 4)
+                  *reinterpret_cast<float4*>(sp + x * G + g) =
+                      *reinterpret_cast<const float4*>(s_p + x * G + g);
+              } else if constexpr (G == 2) {
+                *reinterpret_cast<float2*>(sp + x * 2) = *reinterpret_cast<const float2*>(s_p + x * 2);
+              } else {
+                sp[x] = s_p[x];
+              }
+            }
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) m[g] = -INFINITY;
 #pragma unroll
@@ -1063,6 +1103,7 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[g][e] += __shfl_xor(acc[g][e], o);
   }
+  static_assert(MODE != kScores || SPLIT > 1, "the score builds leave (m, l) in the combine");
   if constexpr (SPLIT == 1 && I8PV) {
     if (kq < G) {
       float mg = m[0], lg = l[0];  // head kq's state
@@ -1198,6 +1239,13 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
       }
       if (nparts == 1) {
         out[(head0 + g) * D + d] = ls > 0.0f ? v / ls : 0.0f;
+        if constexpr (MODE == kScores) {
+          if (d == 0) {
+            const int64_t row = (head0 + g) * max_parts + part;
+            part_ml[row * 2 + 0] = M;
+            part_ml[row * 2 + 1] = ls;
+          }
+        }
       } else {
         const int64_t row = (head0 + g) * max_parts + part;
         part_acc[row * D + d] = v;
@@ -1221,21 +1269,23 @@ constexpr int ring_for() {
 }
 
 template <typename T, int D, int G, int FMT, int NTILE, int SPLIT = split_of<T>()>
-Launch make_launch(bool append) {
+Launch make_launch(DecodeMode mode) {
+  constexpr int R = ring_for<T, D, NTILE, SPLIT>();
   Launch l;
   l.nw = SPLIT;
-  if constexpr (FMT == RKV_BF16 || FMT == RKV_I8 || FMT == RKV_FP8) {  // fused append builds
-    if (append) {
-      l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, ring_for<T, D, NTILE, SPLIT>(),
-                                       SPLIT, FMT, true>;
-      return l;
-    }
-  } else if (append) {
-    return Launch{};
+  if (mode == kAppend) {
+    if constexpr (FMT == RKV_BF16 || FMT == RKV_I8 || FMT == RKV_FP8)
+      l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, R, SPLIT, FMT, kAppend>;
+  } else if (mode == kScores) {
+    // the 8-wave builds and the ones between the smallest and the small
+    // partition have no score form (pick_p asks for none)
+    if constexpr (SPLIT == split_of<T>() && (NTILE == kShortP / kBS || NTILE == kSmallP / kBS ||
+                                             NTILE == part_of<T>() / kBS))
+      l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, R, SPLIT, FMT, kScores>;
+  } else {
+    l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, R, SPLIT, FMT>;
   }
-  l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, ring_for<T, D, NTILE, SPLIT>(), SPLIT,
-                                   FMT>;
-  return l;
+  return l.kernel ? l : Launch{};
 }
 
 // The build for partitions of P tokens: above the largest 4-wave build (bf16
@@ -1250,42 +1300,46 @@ Launch make_launch(bool append) {
 // waves on the same tokens are slower (100 tokens 6.9 against 6.4 with 256
 // token slots), and so is a deeper ring below 200 sequences.
 template <typename T, int D, int G, int FMT>
-Launch pick_p(int P, bool append) {
+Launch pick_p(int P, DecodeMode mode) {
   if constexpr (FMT == RKV_BF16) {
     if (P > kP) {
-      if (P <= kWideP1) return make_launch<T, D, G, FMT, kWideP1 / kBS, kWideSplit>(append);
-      return make_launch<T, D, G, FMT, kWideP2 / kBS, kWideSplit>(append);
+      if (P <= kWideP1) return make_launch<T, D, G, FMT, kWideP1 / kBS, kWideSplit>(mode);
+      return make_launch<T, D, G, FMT, kWideP2 / kBS, kWideSplit>(mode);
     }
   }
-  if (P <= kShortP) return make_launch<T, D, G, FMT, kShortP / kBS>(append);
-  if (P <= 2 * kShortP) return make_launch<T, D, G, FMT, 2 * kShortP / kBS>(append);
-  if (P <= 3 * kShortP) return make_launch<T, D, G, FMT, 3 * kShortP / kBS>(append);
-  if constexpr (kSmallP < part_of<T>()) {
-    if (P <= kSmallP) return make_launch<T, D, G, FMT, kSmallP / kBS>(append);
+  if (P <= kShortP) return make_launch<T, D, G, FMT, kShortP / kBS>(mode);
+  if (mode == kScores) {
+    if (P <= kSmallP) return make_launch<T, D, G, FMT, kSmallP / kBS>(mode);
+    return make_launch<T, D, G, FMT, part_of<T>() / kBS>(mode);
   }
-  return make_launch<T, D, G, FMT, part_of<T>() / kBS>(append);
+  if (P <= 2 * kShortP) return make_launch<T, D, G, FMT, 2 * kShortP / kBS>(mode);
+  if (P <= 3 * kShortP) return make_launch<T, D, G, FMT, 3 * kShortP / kBS>(mode);
+  if constexpr (kSmallP < part_of<T>()) {
+    if (P <= kSmallP) return make_launch<T, D, G, FMT, kSmallP / kBS>(mode);
+  }
+  return make_launch<T, D, G, FMT, part_of<T>() / kBS>(mode);
 }
 
 template <typename T, int D, int FMT>
-Launch pick_g(int G, int P, bool append) {
+Launch pick_g(int G, int P, DecodeMode mode) {
   switch (G) {
-    case 1: return pick_p<T, D, 1, FMT>(P, append);
-    case 2: return pick_p<T, D, 2, FMT>(P, append);
-    case 4: return pick_p<T, D, 4, FMT>(P, append);
-    case 8: return pick_p<T, D, 8, FMT>(P, append);
+    case 1: return pick_p<T, D, 1, FMT>(P, mode);
+    case 2: return pick_p<T, D, 2, FMT>(P, mode);
+    case 4: return pick_p<T, D, 4, FMT>(P, mode);
+    case 8: return pick_p<T, D, 8, FMT>(P, mode);
     default: return Launch{};
   }
 }
 
 // 16-bit and fp32 pools: head_dim 32, 64, 128; 1-byte pools: 64, 128.
 template <typename T, int FMT>
-Launch pick_d(int D, int G, int P, bool append) {
+Launch pick_d(int D, int G, int P, DecodeMode mode) {
   switch (D) {
     case 32:
       if constexpr (sizeof(T) == 1) return Launch{};
-      else return pick_g<T, 32, FMT>(G, P, append);
-    case 64: return pick_g<T, 64, FMT>(G, P, append);
-    case 128: return pick_g<T, 128, FMT>(G, P, append);
+      else return pick_g<T, 32, FMT>(G, P, mode);
+    case 64: return pick_g<T, 64, FMT>(G, P, mode);
+    case 128: return pick_g<T, 128, FMT>(G, P, mode);
     default: return Launch{};
   }
 }

@@ -1,0 +1,435 @@
+// evict.hip -- eviction by accumulated attention weight: which rows of a
+// sequence each KV head keeps (rkv_evict_select), and their move to the blocks
+// of a new table (rkv_evict_compact).  The sums come from
+// rkv_decode_attention_weights (paged_decode.hip).
+#include "block_quant.hpp"
+
+namespace rkv {
+namespace {
+
+constexpr int kBS = 16;
+
+// ---- select --------------------------------------------------------------------
+// One workgroup per (layer, sequence, KV head).  Every position becomes a 32-bit
+// key that orders like (class, weight): 0 absent, 1 a NaN sum, then the sums in
+// float order, all ones the first and last positions, which are always kept.
+// The n-th largest key is built bit by bit from the top: a bit stays set if at
+// least n keys reach the candidate, so 32 counts at most, fewer when a candidate
+// is reached by exactly n.  A count is a ballot per four keys and a sum over the
+// waves in LDS; the keys stay in registers (J groups of four a thread), or are
+// read again for each count where a context is longer than the registers hold
+// (J = 0).
+// Positions are then taken in order: a key above the threshold is kept, one that
+// equals it while the count lasts, so ties go to the lower position.  With both
+// counts in one prefix sum, the place of a position is
+//   (above before it) + min(equal before it, equal wanted).
+// Thread t of NT holds positions 4 (t + NT j) .. + 3, a float4 of one block.
+
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  const uint32_t u = __float_as_uint(w + 0.0f);  // -0 and +0 are one weight
+  const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return w == w ? k : 1u;
+}
+
+template <int NT, int J>
+__global__ __launch_bounds__(NT) void evict_select_kernel(
+    int32_t* __restrict__ keep, int32_t* __restrict__ new_lens,
+    const float* __restrict__ weights, int64_t weights_layer_stride,
+    const int32_t* __restrict__ block_tables, int max_blocks_per_seq,
+    const int32_t* __restrict__ ctx_lens, int num_kv_heads, int64_t num_blocks, int budget,
+    int sinks, int recent, int cap) {
+  constexpr int NW = NT / 64;
+  constexpr int JR = J ? J : 1;
+  __shared__ int s_cnt[2][NW];
+  const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int L = ctx_lens[b];
+  L = L < 0 ? 0 : (L > cap ? cap : L);
+  const int32_t* __restrict__ tab = block_tables + (int64_t)b * max_blocks_per_seq;
+  const float* __restrict__ wl = weights + layer * weights_layer_stride;
+  const int groups = (L + 3) / 4;
+  const int nj = (groups + NT - 1) / NT;
+
+  auto load_keys = [&](int j, uint32_t (&k)[4]) {
+    const int g = tid + NT * j, p = 4 * g;
+    k[0] = k[1] = k[2] = k[3] = 0u;
+    if (g < groups) {
+      const int32_t blk = tab[p / kBS];
+      if (blk >= 0 && blk < num_blocks) {
+        const float4 v = *reinterpret_cast<const float4*>(
+            wl + ((int64_t)blk * num_kv_heads + h) * kBS + p % kBS);
+        const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int q = p + e;
+          const bool held = q < sinks || q >= L - recent;
+          k[e] = q < L ? (held ? 0xffffffffu : weight_key(vv[e])) : 0u;
+        }
+      }
+    }
+  };
+  uint32_t key[JR][4];
+  if constexpr (J > 0) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) load_keys(j, key[j]);
+  }
+  auto for_keys = [&](auto&& f) __attribute__((always_inline)) {
+    if constexpr (J > 0) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) f(j, key[j]);
+    } else {
+      for (int j = 0; j < nj; ++j) {
+        uint32_t k[4];
+        load_keys(j, k);
+        f(j, k);
+      }
+    }
+  };
+  int buf = 0;
+  // Keys >= t in the workgroup, the same in every thread.
+  auto count = [&](uint32_t t) {
+    int c = 0;
+    for_keys([&](int, const uint32_t (&k)[4]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c += __popcll(__builtin_amdgcn_ballot_w64(k[e] >= t));
+    });
+    if (lane == 0) s_cnt[buf][w] = c;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) all += s_cnt[buf][x];
+    buf ^= 1;  // the next count writes the other row: one barrier a count
+    return all;
+  };
+
+  const int present = count(1u);
+  const int n = present < budget ? present : budget;
+  if (h == 0 && layer == 0 && tid == 0) new_lens[b] = n;
+  uint32_t thr = 1u;
+  int reach = present;  // keys >= thr
+  if (present > n && n > 0) {
+    thr = 0u;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = thr | (1u << bit);
+      const int c = count(cand);
+      if (c >= n) {
+        thr = cand;
+        reach = c;
+        if (c == n) break;
+      }
+    }
+  }
+  // wanted among the keys that equal thr (all of them where reach == n)
+  int above = n;
+  if (reach > n) above = thr == 0xffffffffu ? 0 : count(thr + 1u);
+  const int equal = reach > n ? n - above : 0x7fffffff;
+
+  int32_t* __restrict__ out =
+      keep + (((int64_t)layer * gridDim.y + b) * num_kv_heads + h) * budget;
+  __shared__ uint2 s_scan[2][NW];
+  int a0 = 0, e0 = 0;  // above / equal before this chunk
+  int par = 0;
+  if (n > 0) {
+    for_keys([&](int j, const uint32_t (&k)[4]) {
+      if (j >= nj) return;  // workgroup-uniform
+      uint32_t na = 0, ne = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        na += k[e] > thr ? 1u : 0u;
+        ne += k[e] == thr ? 1u : 0u;
+      }
+      uint32_t pa = na, pe = ne;  // inclusive over the wave
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t ua = __shfl_up(pa, o), ue = __shfl_up(pe, o);
+        if (lane >= o) pa += ua, pe += ue;
+      }
+      if (lane == 63) s_scan[par][w] = make_uint2(pa, pe);
+      __syncthreads();
+      uint32_t ba = 0, be = 0, ta = 0, te = 0;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        const uint2 v = s_scan[par][x];
+        if (x < w) ba += v.x, be += v.y;
+        ta += v.x, te += v.y;
+      }
+      par ^= 1;
+      int xa = a0 + (int)(ba + pa - na), xe = e0 + (int)(be + pe - ne);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool up = k[e] > thr, eq = k[e] == thr;
+        if (up || (eq && xe < equal)) out[xa + (xe < equal ? xe : equal)] = 4 * (tid + NT * j) + e;
+        xa += up ? 1 : 0;
+        xe += eq ? 1 : 0;
+      }
+      a0 += (int)ta;
+      e0 += (int)te;
+    });
+  }
+  for (int i = n + tid; i < budget; i += NT) out[i] = -1;
+}
+
+// ---- compact --------------------------------------------------------------------
+// One wave per (layer, sequence, KV head, destination block): lanes 0 .. 15 look
+// up where the block's 16 rows come from, then the wave moves the rows of K and
+// V 16 bytes a lane, all loads issued before the first store.  UPR: 16-byte
+// units a row (template for the unrolled builds, 0: any).  Rows are 128 to 512
+// bytes at scattered places, so whole rows are what memory is asked for.
+template <int DT>
+constexpr bool row_scales() { return DT == RKV_I8 || DT == RKV_FP8; }
+template <int DT>
+constexpr bool tile_scales() { return DT == RKV_I8_BLOCK || DT == RKV_FP8_BLOCK; }
+
+template <int DT, int UPR>
+__global__ __launch_bounds__(256) void evict_compact_kernel(
+    uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, float* __restrict__ k_scale,
+    float* __restrict__ v_scale, float* __restrict__ weights, int64_t layer_bytes,
+    int64_t scale_layer_stride, int64_t weights_layer_stride, const int32_t* __restrict__ keep,
+    const int32_t* __restrict__ new_lens, int budget, const int32_t* __restrict__ src_tables,
+    int src_blocks, const int32_t* __restrict__ dst_tables, int dst_blocks, int num_kv_heads,
+    int upr_any, int64_t num_blocks) {
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + w;
+  const int j = (int)(unit / num_kv_heads), h = (int)(unit - (int64_t)j * num_kv_heads);
+  const int b = blockIdx.y, layer = blockIdx.z;
+  int n = new_lens[b];
+  n = n > budget ? budget : n;
+  if (j >= dst_blocks || (int64_t)j * kBS >= n) return;
+  const int32_t dst = dst_tables[(int64_t)b * dst_blocks + j];
+  if (dst < 0 || dst >= num_blocks) return;
+  // source row (in rows of the layer's pool) of destination row lane, or -1
+  const int row = lane & 15;
+  int64_t from = -1;
+  int32_t sblk = -1;
+  if (j * kBS + row < n) {
+    const int32_t p = keep[(((int64_t)layer * gridDim.y + b) * num_kv_heads + h) * budget +
+                           j * kBS + row];
+    if (p >= 0 && p < src_blocks * kBS) {
+      sblk = src_tables[(int64_t)b * src_blocks + p / kBS];
+      if (sblk >= 0 && sblk < num_blocks)
+        from = ((int64_t)sblk * num_kv_heads + h) * kBS + p % kBS;
+    }
+  }
+  const bool live = from >= 0;
+  const int64_t to = ((int64_t)dst * num_kv_heads + h) * kBS;
+  if (weights && lane < kBS && live) {
+    float* wl = weights + layer * weights_layer_stride;
+    wl[to + row] = wl[from];
+  }
+  float ks = 0.0f, vs = 0.0f, kt = 0.0f, vt = 0.0f;  // source row's scale, the tile's
+  if constexpr (row_scales<DT>()) {
+    if (lane < kBS && live) {
+      float* kl = k_scale + layer * scale_layer_stride;
+      float* vl = v_scale + layer * scale_layer_stride;
+      kl[to + row] = kl[from];
+      vl[to + row] = vl[from];
+    }
+  } else if constexpr (tile_scales<DT>()) {
+    float* kl = k_scale + layer * scale_layer_stride;
+    float* vl = v_scale + layer * scale_layer_stride;
+    if (live) {
+      const int64_t tile = (int64_t)sblk * num_kv_heads + h;
+      ks = kl[tile];
+      vs = vl[tile];
+    }
+    kt = group_max<16>(ks);  // every 16-lane row holds the same 16 rows
+    vt = group_max<16>(vs);
+    const bool any = __builtin_amdgcn_ballot_w64(live) != 0;
+    if (lane == 0 && any) {
+      const int64_t tile = (int64_t)dst * num_kv_heads + h;
+      kl[tile] = kt;
+      vl[tile] = vt;
+    }
+  }
+  const int upr = UPR ? UPR : upr_any;  // 16-byte units a row
+  const int64_t rb = (int64_t)upr * 16;
+  uint8_t* kp = k_pool + layer * layer_bytes;
+  uint8_t* vp = v_pool + layer * layer_bytes;
+  auto convert = [&](uint4 x, float s, float t) {
+    if constexpr (tile_scales<DT>()) {
+      if (s != t) {
+        const float ratio = s / t;  // t > s >= 0
+        x.x = tile_reword<DT>(x.x, s, t, ratio);
+        x.y = tile_reword<DT>(x.y, s, t, ratio);
+        x.z = tile_reword<DT>(x.z, s, t, ratio);
+        x.w = tile_reword<DT>(x.w, s, t, ratio);
+      }
+    }
+    return x;
+  };
+  auto shfl64 = [&](int64_t v, int src) {
+    const int lo = __shfl((int)(uint32_t)v, src), hi = __shfl((int)(v >> 32), src);
+    return ((int64_t)hi << 32) | (uint32_t)lo;
+  };
+  if constexpr (UPR > 0) {
+    constexpr int NU = kBS * UPR;                 // units of a tile
+    constexpr int NP = NU >= 64 ? NU / 64 : 1;    // passes
+    uint4 xk[NP], xv[NP];
+    int64_t src[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int u = lane + 64 * i;
+      const int r = u / UPR < kBS ? u / UPR : kBS - 1;
+      src[i] = shfl64(from, r);
+      if (u >= NU) src[i] = -1;
+      if (src[i] >= 0) {
+        xk[i] = load_stream(kp + src[i] * rb + (u % UPR) * 16);
+        xv[i] = load_stream(vp + src[i] * rb + (u % UPR) * 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int u = lane + 64 * i;
+      const int r = u / UPR < kBS ? u / UPR : kBS - 1;
+      float sk = 0.0f, sv = 0.0f;
+      if constexpr (tile_scales<DT>()) {
+        sk = __shfl(ks, r);
+        sv = __shfl(vs, r);
+      }
+      if (src[i] >= 0) {
+        store_stream(kp + (to + r) * rb + (u % UPR) * 16, convert(xk[i], sk, kt));
+        store_stream(vp + (to + r) * rb + (u % UPR) * 16, convert(xv[i], sv, vt));
+      }
+    }
+  } else {
+    for (int r = 0; r < kBS; ++r) {
+      const int64_t src = shfl64(from, r);
+      if (src < 0) continue;  // wave-uniform
+      for (int u = lane; u < upr; u += 64) {
+        const uint4 a = load_stream(kp + src * rb + u * 16);
+        const uint4 c = load_stream(vp + src * rb + u * 16);
+        store_stream(kp + (to + r) * rb + u * 16, a);
+        store_stream(vp + (to + r) * rb + u * 16, c);
+      }
+    }
+  }
+}
+
+}  // namespace
+}  // namespace rkv
+
+using namespace rkv;
+
+extern "C" int rkv_evict_select(int32_t* keep, int32_t* new_lens, const float* weights,
+                                int64_t weights_layer_stride, const int32_t* block_tables,
+                                int max_blocks_per_seq, const int32_t* ctx_lens, int num_seqs,
+                                int n_layers, int num_kv_heads, int block_size,
+                                int64_t num_blocks, int budget, int sinks, int recent,
+                                int max_context, void* stream) {
+  clear_error();
+  if (num_seqs < 0 || n_layers < 0 || num_kv_heads <= 0 || num_blocks < 0 ||
+      max_blocks_per_seq < 0 || max_context < 0)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_select: bad size argument");
+  if (block_size != kBS)
+    return fail(RKV_ERR_UNSUPPORTED, "rkv_evict_select: block_size must be 16");
+  if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+    return fail(RKV_ERR_INVALID_ARG,
+                "rkv_evict_select: budget must be > 0 and hold sinks + recent rows");
+  if (num_seqs > 65535 || n_layers > 65535)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_select: num_seqs and n_layers must be <= 65535");
+  if ((int64_t)max_blocks_per_seq * kBS > 0x7fffff00)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_select: max_blocks_per_seq too large");
+  if (num_seqs == 0 || n_layers == 0) return RKV_OK;
+  if (!keep || !new_lens || !ctx_lens || (max_blocks_per_seq > 0 && (!weights || !block_tables)))
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_select: null pointer argument");
+  if (!aligned16(weights) || (n_layers > 1 && (weights_layer_stride & 3)))
+    return fail(RKV_ERR_INVALID_ARG,
+                "rkv_evict_select: weights must be 16-byte aligned, its layer stride a multiple of 4");
+  const int table = max_blocks_per_seq * kBS;
+  const int cap = max_context < table ? max_context : table;
+  const dim3 grid((unsigned)num_kv_heads, (unsigned)num_seqs, (unsigned)n_layers);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define RKV_SELECT(NT, J)                                                                        \
+  evict_select_kernel<NT, J><<<grid, NT, 0, s>>>(keep, new_lens, weights, weights_layer_stride,  \
+                                                 block_tables, max_blocks_per_seq, ctx_lens,     \
+                                                 num_kv_heads, num_blocks, budget, sinks, recent, cap)
+  if (cap <= 1024) RKV_SELECT(256, 1);
+  else if (cap <= 4096) RKV_SELECT(1024, 1);
+  else if (cap <= 16384) RKV_SELECT(1024, 4);
+  else if (cap <= 65536) RKV_SELECT(1024, 16);
+  else RKV_SELECT(1024, 0);
+#undef RKV_SELECT
+  return check_launch("rkv_evict_select");
+}
+
+extern "C" int rkv_evict_compact(void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                                 float* weights, int64_t pool_layer_stride,
+                                 int64_t weights_layer_stride, const int32_t* keep,
+                                 const int32_t* new_lens, int budget, const int32_t* src_tables,
+                                 int src_blocks_per_seq, const int32_t* dst_tables,
+                                 int dst_blocks_per_seq, int num_seqs, int n_layers,
+                                 int num_kv_heads, int head_dim, int block_size,
+                                 int64_t num_blocks, int dtype, void* stream) {
+  clear_error();
+  if (num_seqs < 0 || n_layers < 0 || num_kv_heads <= 0 || num_blocks < 0 || budget <= 0 ||
+      src_blocks_per_seq < 0 || dst_blocks_per_seq < 0)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_compact: bad size argument");
+  if (dtype < RKV_F32 || dtype > RKV_FP8_BLOCK)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_compact: unknown dtype");
+  const bool q8 = dtype >= RKV_I8;
+  if (block_size != kBS)
+    return fail(RKV_ERR_UNSUPPORTED, "rkv_evict_compact: block_size must be 16");
+  if (q8 ? head_dim != 32 && head_dim != 64 && head_dim != 128 : head_dim <= 0 || head_dim % 8)
+    return fail(RKV_ERR_UNSUPPORTED,
+                "rkv_evict_compact: head_dim must be a multiple of 8 (1-byte pools: 32, 64, 128)");
+  if (num_seqs > 65535 || n_layers > 65535)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_compact: num_seqs and n_layers must be <= 65535");
+  if ((int64_t)src_blocks_per_seq * kBS > 0x7fffff00)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_compact: src_blocks_per_seq too large");
+  if (num_seqs == 0 || n_layers == 0 || src_blocks_per_seq == 0 || dst_blocks_per_seq == 0)
+    return RKV_OK;
+  if (!k_pool || !v_pool || !keep || !new_lens || !src_tables || !dst_tables ||
+      (q8 && (!k_scale || !v_scale)))
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_compact: null pointer argument");
+  if (!aligned16(k_pool) || !aligned16(v_pool))
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_compact: pools must be 16-byte aligned");
+  const int elem = dtype == RKV_F32 ? 4 : dtype == RKV_BF16 ? 2 : 1;
+  const int64_t row_bytes = (int64_t)head_dim * elem;
+  const int64_t layer_bytes = n_layers > 1 ? pool_layer_stride * elem : 0;
+  if (layer_bytes % 16)
+    return fail(RKV_ERR_INVALID_ARG,
+                "rkv_evict_compact: a layer must start on a multiple of 16 bytes");
+  const int64_t per_scale = dtype == RKV_I8 || dtype == RKV_FP8 ? head_dim : kBS * head_dim;
+  const int64_t scale_ls = n_layers > 1 && q8 ? pool_layer_stride / per_scale : 0;
+  if (n_layers > 1 && q8 && pool_layer_stride % per_scale)
+    return fail(RKV_ERR_INVALID_ARG,
+                "rkv_evict_compact: pool_layer_stride must be a whole number of scales");
+  int64_t blocks = (budget + (int64_t)kBS - 1) / kBS;
+  if (blocks > dst_blocks_per_seq) blocks = dst_blocks_per_seq;
+  const int64_t wgs = (blocks * num_kv_heads + 3) / 4;
+  if (wgs > 0x7fffffff)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_evict_compact: budget too large for one launch");
+  const dim3 grid((unsigned)wgs, (unsigned)num_seqs, (unsigned)n_layers);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int upr = (int)(row_bytes / 16);
+#define RKV_COMPACT(T, U)                                                                      \
+  evict_compact_kernel<T, U><<<grid, 256, 0, s>>>(                                             \
+      static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), k_scale, v_scale, weights, \
+      layer_bytes, scale_ls, weights_layer_stride, keep, new_lens, budget, src_tables,         \
+      src_blocks_per_seq, dst_tables, dst_blocks_per_seq, num_kv_heads, upr, num_blocks)
+#define RKV_COMPACT_Q(T)                   \
+  do {                                     \
+    if (upr == 2) RKV_COMPACT(T, 2);       \
+    else if (upr == 4) RKV_COMPACT(T, 4);  \
+    else RKV_COMPACT(T, 8);                \
+  } while (0)
+  switch (dtype) {
+    case RKV_F32:
+    case RKV_BF16:  // rows of bytes: the element type does not matter
+      if (upr == 4) RKV_COMPACT(RKV_F32, 4);
+      else if (upr == 8) RKV_COMPACT(RKV_F32, 8);
+      else if (upr == 16) RKV_COMPACT(RKV_F32, 16);
+      else if (upr == 32) RKV_COMPACT(RKV_F32, 32);
+      else RKV_COMPACT(RKV_F32, 0);
+      break;
+    case RKV_I8:
+    case RKV_FP8: RKV_COMPACT_Q(RKV_I8); break;
+    case RKV_I8_BLOCK: RKV_COMPACT_Q(RKV_I8_BLOCK); break;
+    default: RKV_COMPACT_Q(RKV_FP8_BLOCK); break;
+  }
+#undef RKV_COMPACT_Q
+#undef RKV_COMPACT
+  return check_launch("rkv_evict_compact");
+}

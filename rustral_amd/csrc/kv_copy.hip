@@ -384,7 +384,8 @@ __global__ __launch_bounds__(256) void append_q_kernel(
 #define RKV_GATHER_Q_THREADS 128  // threads per workgroup = words per piece
 #endif
 constexpr int kGatherQThreads = RKV_GATHER_Q_THREADS;
-template <int D, int FMT, int HPW>
+// FORMAT: row-scaled, or the formats with one scale a (block, head) tile.
+template <int D, int FORMAT, int HPW>
 __global__ __launch_bounds__(kGatherQThreads) void gather_q_kernel(
     float* __restrict__ k_out, float* __restrict__ v_out, const uint8_t* __restrict__ k_pool,
     const uint8_t* __restrict__ v_pool, const float* __restrict__ k_scale,
@@ -392,6 +393,8 @@ __global__ __launch_bounds__(kGatherQThreads) void gather_q_kernel(
     int max_blocks_per_seq, const int32_t* __restrict__ ctx_lens,
     const int64_t* __restrict__ out_offsets, int num_kv_heads, int block_size, int ppt,
     int64_t num_blocks, int max_ctx) {
+  constexpr bool TSC = FORMAT == RKV_I8_BLOCK || FORMAT == RKV_FP8_BLOCK;
+  constexpr int FMT = FORMAT == RKV_I8_BLOCK ? RKV_I8 : FORMAT == RKV_FP8_BLOCK ? RKV_FP8 : FORMAT;
   const int ppb = (num_kv_heads / HPW) * ppt;
   const int j = blockIdx.x / ppb;
   const int rem = blockIdx.x - j * ppb;
@@ -423,14 +426,14 @@ __global__ __launch_bounds__(kGatherQThreads) void gather_q_kernel(
   const int u = piece * kGatherQThreads + threadIdx.x;
   const int uc = u < tu ? u : tu - 1;  // loads are unconditional (the tile's last word)
   const uint32_t* src = reinterpret_cast<const uint32_t*>((is_v ? v_pool : k_pool) + row0 * D);
-  const float* sc = (is_v ? v_scale : k_scale) + row0;
+  const float* sc = (is_v ? v_scale : k_scale) + (TSC ? (int64_t)blk * num_kv_heads + h0 : row0);
   uint32_t w[HPW];
   float sk[HPW];
 #pragma unroll
   for (int k = 0; k < HPW; ++k) {
     if constexpr (RKV_GATHER_Q_NTL) w[k] = __builtin_nontemporal_load(src + k * tu + uc);
     else w[k] = src[k * tu + uc];
-    sk[k] = sc[k * block_size + uc / U];
+    sk[k] = sc[TSC ? k : k * block_size + uc / U];
   }
   const int rr = u / U, c = u - rr * U;
   if (u < tu && rr < nt) {
@@ -638,7 +641,11 @@ extern "C" int rkv_gather_q(float* k_out, float* v_out, const void* k_pool, cons
                             int num_kv_heads, int head_dim, int block_size, int64_t num_blocks,
                             int max_ctx, int dtype, void* stream) {
   clear_error();
-  if (int rc = check_q(num_kv_heads, head_dim, block_size, num_blocks, dtype)) return rc;
+  const bool tsc = dtype == RKV_I8_BLOCK || dtype == RKV_FP8_BLOCK;
+  if (int rc = check_q(num_kv_heads, head_dim, block_size, num_blocks, tsc ? dtype - 2 : dtype))
+    return rc;
+  if (tsc && block_size != 16)
+    return fail(RKV_ERR_UNSUPPORTED, "block-scaled pools: block_size must be 16");
   if (num_seqs < 0 || max_blocks_per_seq < 0)
     return fail(RKV_ERR_INVALID_ARG, "negative num_seqs/max_blocks_per_seq");
   if (num_seqs == 0 || max_blocks_per_seq == 0) return RKV_OK;
@@ -672,15 +679,19 @@ extern "C" int rkv_gather_q(float* k_out, float* v_out, const void* k_pool, cons
     else if (hpw == 2) RKV_GATHER_QH(D, F, (RKV_GATHER_Q_HPW > 2 ? 2 : 1));  \
     else RKV_GATHER_QH(D, F, 1);                                             \
   } while (0)
-  if (dtype == RKV_I8) {
-    if (head_dim == 32) RKV_GATHER_Q(32, RKV_I8);
-    else if (head_dim == 64) RKV_GATHER_Q(64, RKV_I8);
-    else RKV_GATHER_Q(128, RKV_I8);
-  } else {
-    if (head_dim == 32) RKV_GATHER_Q(32, RKV_FP8);
-    else if (head_dim == 64) RKV_GATHER_Q(64, RKV_FP8);
-    else RKV_GATHER_Q(128, RKV_FP8);
+#define RKV_GATHER_QD(F)                            \
+  do {                                              \
+    if (head_dim == 32) RKV_GATHER_Q(32, F);        \
+    else if (head_dim == 64) RKV_GATHER_Q(64, F);   \
+    else RKV_GATHER_Q(128, F);                      \
+  } while (0)
+  switch (dtype) {
+    case RKV_I8: RKV_GATHER_QD(RKV_I8); break;
+    case RKV_FP8: RKV_GATHER_QD(RKV_FP8); break;
+    case RKV_I8_BLOCK: RKV_GATHER_QD(RKV_I8_BLOCK); break;
+    default: RKV_GATHER_QD(RKV_FP8_BLOCK); break;
   }
+#undef RKV_GATHER_QD
 #undef RKV_GATHER_Q
 #undef RKV_GATHER_QH
   return check_launch("rkv_gather_q");

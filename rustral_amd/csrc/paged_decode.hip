@@ -228,9 +228,71 @@ __global__ __launch_bounds__(256) void decode_merge_rows_kernel(
   }
 }
 
+// ---- accumulated weights -------------------------------------------------------
+// Pass 3 of rkv_decode_attention_weights: the partition pass left every score
+// (log2 domain) and every partition's (m, l); a row's weight is
+//   sum over the group's heads of 2^(score - M_h) / l_h,
+//   M_h = max m_p,  l_h = sum 2^(m_p - M_h) l_p.
+// grid = (chunks of kWeightTokens positions, KV heads, sequences): every
+// workgroup settles its G heads' (M, 1 / l) from the partitions, then a thread
+// takes whole positions (G scores, one 4 G-byte load) and adds their weight to
+// the row's sum.  The adds are hardware atomics: a block of several sequences
+// (a shared prefix) loses none, any other row has a single adder.
+constexpr int kWeightTokens = 1024;
+
+template <int G>
+__global__ __launch_bounds__(256) void decode_weights_kernel(
+    float* __restrict__ weights, const float* __restrict__ scores,
+    const float* __restrict__ part_ml, const int32_t* __restrict__ block_tables,
+    int max_blocks_per_seq, const int32_t* __restrict__ ctx_lens, int ctx_cap, int num_kv_heads,
+    int64_t num_blocks, int P, int max_parts) {
+  __shared__ float s_m[G], s_inv[G];
+  const int kh = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int L = ctx_lens[b];
+  L = L < 0 ? 0 : (L > ctx_cap ? ctx_cap : L);
+  const int t0 = blockIdx.x * kWeightTokens;
+  if (t0 >= L) return;
+  const int np = (L + P - 1) / P;
+  for (int g = w; g < G; g += 4) {  // a wave a head
+    const float* ml =
+        part_ml + (((int64_t)b * num_kv_heads + kh) * G + g) * max_parts * 2;
+    float M = -INFINITY;
+    for (int p = lane; p < np; p += 64) M = fmaxf(M, ml[2 * p]);
+    M = wave_max(M);
+    float l = 0.0f;
+    for (int p = lane; p < np; p += 64)
+      l += ml[2 * p] == -INFINITY ? 0.0f : exp2f(ml[2 * p] - M) * ml[2 * p + 1];
+    l = wave_sum(l);
+    if (lane == 0) {
+      s_m[g] = M;
+      s_inv[g] = l > 0.0f ? 1.0f / l : 0.0f;
+    }
+  }
+  __syncthreads();
+  float M[G], inv[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) M[g] = s_m[g], inv[g] = s_inv[g];
+  const float* sp =
+      scores + (((int64_t)b * num_kv_heads + kh) * ((int64_t)max_parts * P)) * G;
+  const int32_t* tab = block_tables + (int64_t)b * max_blocks_per_seq;
+  const int t1 = L < t0 + kWeightTokens ? L : t0 + kWeightTokens;
+  for (int t = t0 + tid; t < t1; t += 256) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float s = sp[(int64_t)t * G + g];
+      sum += s == -INFINITY ? 0.0f : exp2f(s - M[g]) * inv[g];
+    }
+    const int32_t blk = tab[t / kBS];
+    if (blk >= 0 && blk < num_blocks)
+      unsafeAtomicAdd(weights + ((int64_t)blk * num_kv_heads + kh) * kBS + t % kBS, sum);
+  }
+}
+
 // ---- dispatch ----------------------------------------------------------------
 
-inline bool one_byte(int dtype) { return dtype == RKV_I8 || dtype == RKV_FP8; }
+inline bool one_byte(int dtype) { return dtype >= RKV_I8 && dtype <= RKV_FP8_BLOCK; }
 
 int default_part(int dtype, int /*max_context*/) { return one_byte(dtype) ? kPQ : kP; }
 
@@ -314,12 +376,14 @@ int resolve_part(int requested, int dtype, int max_context) {
   return RKV_ERR_UNSUPPORTED;
 }
 
-Launch pick(int dtype, int D, int G, int P, bool append) {
+Launch pick(int dtype, int D, int G, int P, DecodeMode mode) {
   switch (dtype) {
-    case RKV_F32: return decode_f32(D, G, P, append);
-    case RKV_BF16: return decode_bf16(D, G, P, append);
-    case RKV_I8: return decode_i8(D, G, P, append);
-    case RKV_FP8: return decode_fp8(D, G, P, append);
+    case RKV_F32: return decode_f32(D, G, P, mode);
+    case RKV_BF16: return decode_bf16(D, G, P, mode);
+    case RKV_I8: return decode_i8(D, G, P, mode);
+    case RKV_FP8: return decode_fp8(D, G, P, mode);
+    case RKV_I8_BLOCK: return decode_i8_block(D, G, P, mode);
+    case RKV_FP8_BLOCK: return decode_fp8_block(D, G, P, mode);
     default: return Launch{};
   }
 }
@@ -340,7 +404,8 @@ struct DecodeArgs {
   void* workspace;
   size_t workspace_bytes;
   hipStream_t stream;
-  const float* k_scale = nullptr;  // 1-byte pools: [num_blocks][Hkv][block_size] fp32
+  const float* k_scale = nullptr;  // 1-byte pools: [num_blocks][Hkv][block_size] fp32, with
+                                   // one scale a tile [num_blocks][Hkv]
   const float* v_scale = nullptr;
   const float* k_new = nullptr;  // fused append (bf16 pools): [num_seqs][Hkv][D] fp32
   const float* v_new = nullptr;
@@ -376,9 +441,9 @@ int validate(const DecodeArgs& a, int& max_parts, int& P) {
     return fail(RKV_ERR_INVALID_ARG, "negative size argument");
   if (a.num_q_heads <= 0 || a.num_kv_heads <= 0 || a.num_q_heads % a.num_kv_heads)
     return fail(RKV_ERR_INVALID_ARG, "num_q_heads must be a positive multiple of num_kv_heads");
-  const bool q8 = a.dtype == RKV_I8 || a.dtype == RKV_FP8;
+  const bool q8 = one_byte(a.dtype);
   if (a.dtype != RKV_F32 && a.dtype != RKV_BF16 && !q8)
-    return fail(RKV_ERR_INVALID_ARG, "dtype must be RKV_F32, RKV_BF16, RKV_I8 or RKV_FP8");
+    return fail(RKV_ERR_INVALID_ARG, "dtype must be RKV_F32, RKV_BF16 or a 1-byte format");
   if (q8 && a.head_dim == 32)
     return fail(RKV_ERR_UNSUPPORTED, "1-byte pools: head_dim must be 64 or 128");
   if (a.block_size != kBS) return fail(RKV_ERR_UNSUPPORTED, "block_size must be 16");
@@ -430,7 +495,7 @@ int launch_partitions(const DecodeArgs& a, int max_parts, int P) {
   // tokens the smallest build that does (pick_p).
   if (max_parts == 1 && cap <= kSmallP)
     P = cap <= kShortP ? kShortP : (cap + kShortP - 1) / kShortP * kShortP;
-  Launch l = pick(a.dtype, a.head_dim, G, P, a.k_new != nullptr);
+  Launch l = pick(a.dtype, a.head_dim, G, P, a.k_new ? kAppend : kAttend);
   if (!l.kernel) return fail(RKV_ERR_UNSUPPORTED, "no decode kernel for this shape");
   float *acc = nullptr, *ml = nullptr;
   if (max_parts > 1) split_ws(a.workspace, a.num_seqs, a.num_q_heads, a.head_dim, max_parts, acc, ml);
@@ -441,7 +506,7 @@ int launch_partitions(const DecodeArgs& a, int max_parts, int P) {
                      a.v_pool, a.k_scale, a.v_scale, a.block_tables, a.max_blocks_per_seq,
                      a.ctx_lens, cap,
                      a.num_kv_heads, a.num_blocks, a.scale * kLog2e, max_parts,
-                     P / (kBS * l.nw), a.k_new, a.v_new);
+                     P / (kBS * l.nw), a.k_new, a.v_new, nullptr);
   return check_launch("decode_stream_kernel");
 }
 
@@ -517,7 +582,7 @@ extern "C" int rkv_decode_partition_size(int partition_size, int head_dim, int d
   clear_error();
   (void)head_dim;
   if (dtype != RKV_F32 && dtype != RKV_BF16 && !one_byte(dtype))
-    return fail(RKV_ERR_INVALID_ARG, "dtype must be RKV_F32, RKV_BF16, RKV_I8 or RKV_FP8");
+    return fail(RKV_ERR_INVALID_ARG, "dtype must be RKV_F32, RKV_BF16 or a 1-byte format");
   const int P = resolve_part(partition_size, dtype, max_context);
   if (P < 0)
     return fail(P, "partition_size must be a multiple of 64 tokens up to 640, for bf16 pools also "
@@ -530,7 +595,7 @@ extern "C" int rkv_decode_partition_size_for(int partition_size, int num_seqs, i
                                              int max_context) {
   clear_error();
   if (dtype != RKV_F32 && dtype != RKV_BF16 && !one_byte(dtype))
-    return fail(RKV_ERR_INVALID_ARG, "dtype must be RKV_F32, RKV_BF16, RKV_I8 or RKV_FP8");
+    return fail(RKV_ERR_INVALID_ARG, "dtype must be RKV_F32, RKV_BF16 or a 1-byte format");
   if (partition_size <= 0)
     return shape_part(dtype, num_seqs, num_q_heads, num_kv_heads, head_dim,
                       max_context < 0 ? 0 : max_context);
@@ -784,8 +849,15 @@ extern "C" int rkv_decode_attention_q(float* out, const float* q, const void* k_
                                       int partition_size, void* workspace,
                                       size_t workspace_bytes, void* stream) {
   clear_error();
-  if (dtype != RKV_I8 && dtype != RKV_FP8)
-    return fail(RKV_ERR_INVALID_ARG, "rkv_decode_attention_q: dtype must be RKV_I8 or RKV_FP8");
+  if (!one_byte(dtype))
+    return fail(RKV_ERR_INVALID_ARG, "rkv_decode_attention_q: dtype must be a 1-byte format");
+  // block-scaled pools have no earlier default to keep: the shape's pick
+  if (partition_size <= 0 && (dtype == RKV_I8_BLOCK || dtype == RKV_FP8_BLOCK))
+    partition_size = auto_part(dtype, num_seqs, num_q_heads, num_kv_heads, head_dim,
+                               ctx_cap_of(max_context < 0 ? 0 : max_context,
+                                          max_blocks_per_seq < 0 ? 0 : max_blocks_per_seq,
+                                          block_size),
+                               workspace ? workspace_bytes : 0);
   DecodeArgs a{out, q, k_pool, v_pool, block_tables, max_blocks_per_seq, ctx_lens, num_seqs,
                num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_context, scale,
                dtype, partition_size, workspace, workspace_bytes,
@@ -797,4 +869,110 @@ extern "C" int rkv_decode_attention_q(float* out, const float* q, const void* k_
   const int cap = ctx_cap_of(max_context, max_blocks_per_seq, block_size);
   return launch_merge(out, ctx_lens, num_seqs, num_q_heads, head_dim, cap, P, max_parts,
                       workspace, a.stream);
+}
+
+// ---- decode with accumulated weights -------------------------------------------
+
+namespace {
+
+// The workspace of a call with max_parts partitions of P tokens: acc and (m, l)
+// of every partition (also of a sequence's only one), then the scores.
+struct WeightsWs {
+  size_t ml, scores, total;
+};
+WeightsWs weights_ws(int B, int Hq, int D, int64_t max_parts, int64_t tokens) {
+  const auto pad = [](size_t x) { return (x + 255) & ~size_t(255); };
+  const size_t rows = (size_t)B * Hq * max_parts;
+  WeightsWs w;
+  w.ml = pad(rows * D * sizeof(float));
+  w.scores = w.ml + pad(rows * 2 * sizeof(float));
+  w.total = w.scores + (size_t)B * Hq * tokens * sizeof(float);
+  return w;
+}
+
+// Partition sizes with a score build (decode_stream.hpp): the shape's pick, at
+// most the largest 4-wave build's.
+int weights_part(int dtype, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                 int cap) {
+  if (cap <= kShortP) return kShortP;
+  if (cap <= kSmallP) return kSmallP;
+  const int P = shape_part(dtype, num_seqs, num_q_heads, num_kv_heads, head_dim, cap);
+  return P < kP ? P : kP;
+}
+
+}  // namespace
+
+extern "C" size_t rkv_decode_weights_workspace_bytes(int num_seqs, int num_q_heads,
+                                                     int num_kv_heads, int head_dim,
+                                                     int max_context) {
+  if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context <= 0)
+    return 0;
+  // the most partitions any pick gives a call of up to max_context tokens, and
+  // the scores rounded up to whole partitions
+  const auto parts = [&](int64_t P) { return (max_context + P - 1) / P; };
+  const int64_t groups = (int64_t)num_seqs * num_kv_heads;
+  int64_t tiny = 1;
+  if (max_context > kSmallP && kTinyGroups / groups > 0)
+    tiny = std::min({parts(kShortP), (int64_t)kTinyParts, (int64_t)kTinyGroups / groups});
+  return weights_ws(num_seqs, num_q_heads, head_dim, std::max(parts(kSmallP), tiny),
+                    (int64_t)max_context + kP)
+      .total;
+}
+
+extern "C" int rkv_decode_attention_weights(
+    float* out, float* weights, const float* q, const void* k_pool, const void* v_pool,
+    const float* k_scale, const float* v_scale, const int32_t* block_tables,
+    int max_blocks_per_seq, const int32_t* ctx_lens, int num_seqs, int num_q_heads,
+    int num_kv_heads, int head_dim, int block_size, int64_t num_blocks, int max_context,
+    float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (num_seqs > 0 && !weights)
+    return fail(RKV_ERR_INVALID_ARG, "rkv_decode_attention_weights: null weights");
+  const int cap = ctx_cap_of(max_context < 0 ? 0 : max_context,
+                             max_blocks_per_seq < 0 ? 0 : max_blocks_per_seq, block_size);
+  const int P = weights_part(dtype, num_seqs, num_q_heads, num_kv_heads, head_dim, cap);
+  DecodeArgs a{out, q, k_pool, v_pool, block_tables, max_blocks_per_seq, ctx_lens, num_seqs,
+               num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, max_context, scale,
+               dtype, P, workspace, workspace_bytes, static_cast<hipStream_t>(stream), k_scale,
+               v_scale};
+  int max_parts = 1, P2 = 0;
+  if (int rc = validate(a, max_parts, P2)) return rc;
+  if (num_seqs == 0) return RKV_OK;
+  const WeightsWs ws = weights_ws(num_seqs, num_q_heads, head_dim, max_parts,
+                                  (int64_t)max_parts * P2);
+  if (!workspace || workspace_bytes < ws.total)
+    return fail(RKV_ERR_WORKSPACE,
+                "workspace missing or smaller than rkv_decode_weights_workspace_bytes()");
+  if (!aligned16(workspace))
+    return fail(RKV_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+  const int G = num_q_heads / num_kv_heads;
+  const Launch l = pick(dtype, head_dim, G, P2, kScores);
+  if (!l.kernel) return fail(RKV_ERR_UNSUPPORTED, "no decode kernel for this shape");
+  float* acc = static_cast<float*>(workspace);
+  float* ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.ml);
+  float* scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + ws.scores);
+  const dim3 grid((unsigned)num_kv_heads, (unsigned)max_parts, (unsigned)num_seqs);
+  hipLaunchKernelGGL(l.kernel, grid, dim3(l.nw * 64), 0, a.stream, out, acc, ml, q, k_pool, v_pool,
+                     k_scale, v_scale, block_tables, max_blocks_per_seq, ctx_lens, cap,
+                     num_kv_heads, num_blocks, scale * kLog2e, max_parts, P2 / (kBS * l.nw),
+                     nullptr, nullptr, scores);
+  if (int rc = check_launch("decode_stream_kernel")) return rc;
+  if (int rc = launch_merge(out, ctx_lens, num_seqs, num_q_heads, head_dim, cap, P2, max_parts,
+                            workspace, a.stream))
+    return rc;
+  if (cap <= 0) return RKV_OK;
+  const dim3 wgrid((unsigned)((cap + kWeightTokens - 1) / kWeightTokens), (unsigned)num_kv_heads,
+                   (unsigned)num_seqs);
+#define RKV_WEIGHTS(GG)                                                                         \
+  decode_weights_kernel<GG><<<wgrid, 256, 0, a.stream>>>(weights, scores, ml, block_tables,     \
+                                                         max_blocks_per_seq, ctx_lens, cap,     \
+                                                         num_kv_heads, num_blocks, P2, max_parts)
+  switch (G) {
+    case 1: RKV_WEIGHTS(1); break;
+    case 2: RKV_WEIGHTS(2); break;
+    case 4: RKV_WEIGHTS(4); break;
+    default: RKV_WEIGHTS(8); break;
+  }
+#undef RKV_WEIGHTS
+  return check_launch("decode_weights_kernel");
 }

@@ -278,6 +278,10 @@ def decode_attention_append(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 
 _QFMT = {"int8": _lib.RKV_I8, "fp8": _lib.RKV_FP8, _lib.RKV_I8: _lib.RKV_I8,
          _lib.RKV_FP8: _lib.RKV_FP8}
+# one scale a (block, KV head) tile instead of one a row
+_BFMT = {"int8_block": _lib.RKV_I8_BLOCK, "fp8_block": _lib.RKV_FP8_BLOCK,
+         _lib.RKV_I8_BLOCK: _lib.RKV_I8_BLOCK, _lib.RKV_FP8_BLOCK: _lib.RKV_FP8_BLOCK}
+_ANYFMT = {**_QFMT, **_BFMT}
 
 
 def _qcode(fmt) -> int:
@@ -286,11 +290,34 @@ def _qcode(fmt) -> int:
     return _QFMT[fmt]
 
 
+def _anycode(fmt) -> int:
+    if fmt not in _ANYFMT:
+        raise ValueError(f"1-byte format {fmt!r}: want 'int8', 'fp8', 'int8_block' or "
+                         "'fp8_block'")
+    return _ANYFMT[fmt]
+
+
+def _bcode(fmt) -> int:
+    if fmt not in _BFMT:
+        raise ValueError(f"block-scaled format {fmt!r}: want 'int8_block' or 'fp8_block'")
+    return _BFMT[fmt]
+
+
+def _scale_pools(k_pool, v_pool, k_scale, v_scale, code: int) -> None:
+    """Scale pools of the shape their format has: one a row, or one a tile.  The
+    kernels index them by the byte pools' shape."""
+    _dev(k_scale, "k_scale", torch.float32), _dev(v_scale, "v_scale", torch.float32)
+    cut = -2 if code >= _lib.RKV_I8_BLOCK else -1
+    if k_scale.shape != k_pool.shape[:cut] or v_scale.shape != v_pool.shape[:cut]:
+        raise ValueError("scale pools must be the byte pools' shape without head_dim, and for the "
+                         "block formats without the rows too")
+
+
 def _workspace_bytes_q(num_seqs: int, num_q_heads: int, head_dim: int, max_context: int,
                        size: int, fmt) -> int:
-    """The workspace of a call over 1-byte pools, which take the split entry
-    points' size, not partition_size_for's, where none is asked for."""
-    if size <= 0:
+    """The workspace of a call over 1-byte pools: row-scaled ones take the split
+    entry points' size, not partition_size_for's, where none is asked for."""
+    if size <= 0 and fmt in _QFMT:
         size = partition_size(_qcode(fmt), max_context, head_dim=head_dim)
     return workspace_bytes(num_seqs, num_q_heads, head_dim, max_context, size)
 
@@ -328,7 +355,11 @@ def gather_q(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
     """Dequantized K/V per sequence in fp32: padded [B, Hkv, max_ctx, D], or
     packed (out_offsets int64 [B] given) as flat tensors of out_total
     elements.  Untouched rows keep the contents of k_out/v_out (zeros when
-    allocated here)."""
+    allocated here).  Any 1-byte format; the block formats' scale pools are
+    [num_blocks, Hkv]."""
+    code = _anycode(fmt)
+    if code >= _lib.RKV_I8_BLOCK:
+        _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
     _dev(k_pool, "k_pool", torch.uint8), _dev(v_pool, "v_pool", torch.uint8)
     _dev(k_scale, "k_scale", torch.float32), _dev(v_scale, "v_scale", torch.float32)
     _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
@@ -355,7 +386,7 @@ def gather_q(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
     check(lib().rkv_gather_q(k_out.data_ptr(), v_out.data_ptr(), k_pool.data_ptr(),
                              v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                              block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), off_ptr, B, hkv, d,
-                             bs, nb, max_ctx, _qcode(fmt), _stream(k_pool)))
+                             bs, nb, max_ctx, code, _stream(k_pool)))
     return k_out, v_out
 
 
@@ -406,14 +437,19 @@ def decode_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
                        ctx_lens: torch.Tensor, scale: float | None = None, fmt: str = "int8", *,
                        max_context: int | None = None, out: torch.Tensor | None = None,
                        workspace: torch.Tensor | None = None, partition_size: int = 0) -> torch.Tensor:
-    """decode_attention over 1-byte pools with per-row scales.
-    partition_size 0: 640; partition_size_for gives the size to ask for where a
-    small call wants finer partitions."""
+    """decode_attention over 1-byte pools: per-row scales ('int8', 'fp8'), or one
+    scale a block and KV head ('int8_block', 'fp8_block').
+    partition_size 0: 640 over row-scaled pools, where partition_size_for gives
+    the size to ask for if a small call wants finer partitions; its pick over
+    block-scaled ones."""
+    code = _anycode(fmt)
     _dev(q, "q", torch.float32), _dev(k_pool, "k_pool", torch.uint8)
     _dev(v_pool, "v_pool", torch.uint8), _dev(k_scale, "k_scale", torch.float32)
     _dev(v_scale, "v_scale", torch.float32)
     _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
     nb, hkv, bs, d = k_pool.shape
+    if code >= _lib.RKV_I8_BLOCK:
+        _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
     check_attention_shapes(q.shape, k_pool.shape, block_tables.shape, ctx_lens.shape)
     B, hq, _ = q.shape
     mbs = block_tables.shape[1]
@@ -432,7 +468,7 @@ def decode_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     check(lib().rkv_decode_attention_q(out.data_ptr(), q.data_ptr(), k_pool.data_ptr(),
                                        v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                        block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, hq,
-                                       hkv, d, bs, nb, max_context, float(scale), _qcode(fmt),
+                                       hkv, d, bs, nb, max_context, float(scale), code,
                                        partition_size, ws_ptr, ws_len, _stream(q)))
     return out
 
@@ -468,6 +504,311 @@ def prefill_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
                                       ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, max_q_len,
                                       float(scale), _dtype_code(k_pool), _stream(q)))
     return out
+
+
+def append_block_q(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+                   v_scale: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                   new_start: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+                   fmt: str = "int8_block", *, max_new: int | None = None) -> None:
+    """Quantizing append into pools with one scale a (block, KV head) tile:
+    uint8 [.., nb, Hkv, 16, D] with fp32 scales [.., nb, Hkv].
+
+    k_new / v_new: float32 [total, Hkv, D] or [n_layers, total, Hkv, D]; sequence
+    b's rows are new_start[b] .. new_start[b+1]-1 (int32 [B+1]), the last ones of
+    its ctx_lens[b] tokens.  A block's scale grows to hold its new rows, and its
+    older rows are rounded to it.  max_new bounds every sequence's row count
+    (computed from new_start, with a device sync, when not given).
+    """
+    code = _bcode(fmt)
+    _dev(k_pool, "k_pool", torch.uint8), _dev(v_pool, "v_pool", torch.uint8)
+    _dev(k_new, "k_new", torch.float32), _dev(v_new, "v_new", torch.float32)
+    _dev(new_start, "new_start", torch.int32), _dev(block_tables, "block_tables", torch.int32)
+    _dev(ctx_lens, "ctx_lens", torch.int32)
+    _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
+    multi = k_pool.dim() == 5
+    n_layers = k_pool.shape[0] if multi else 1
+    nb, hkv, bs, d = k_pool.shape[-4:]
+    if k_new.shape != v_new.shape or k_pool.shape != v_pool.shape:
+        raise ValueError("K and V shapes differ")
+    if k_new.shape[-2:] != (hkv, d) or k_new.dim() != (4 if multi else 3) or \
+            (multi and k_new.shape[0] != n_layers):
+        raise ValueError(f"k_new shape {tuple(k_new.shape)} does not match pool {tuple(k_pool.shape)}")
+    B = ctx_lens.shape[0]
+    if ctx_lens.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != B or \
+            new_start.shape != (B + 1,):
+        raise ValueError("one block-table row and one length per sequence, new_start B + 1 offsets")
+    if max_new is None:
+        max_new = int((new_start[1:] - new_start[:-1]).max().item()) if B else 0
+    total = k_new.shape[-3]
+    check(lib().rkv_append_block_q(
+        k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        nb * hkv * bs * d if multi else 0, k_new.data_ptr(), v_new.data_ptr(),
+        total * hkv * d if multi else 0, hkv * d, d, new_start.data_ptr(),
+        block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, n_layers, hkv, d,
+        bs, nb, max_new, code, _stream(k_pool)))
+
+
+def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                        k_scale: torch.Tensor, v_scale: torch.Tensor,
+                        block_tables: torch.Tensor, q_start: torch.Tensor,
+                        ctx_lens: torch.Tensor, scale: float | None = None,
+                        fmt: str = "int8_block", *, max_q_len: int | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """prefill_attention over block-scaled 8-bit pools ('int8_block',
+    'fp8_block')."""
+    code = _bcode(fmt)
+    _dev(q, "q", torch.float32), _dev(k_pool, "k_pool", torch.uint8)
+    _dev(v_pool, "v_pool", torch.uint8), _dev(q_start, "q_start", torch.int32)
+    _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
+    _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
+    check_attention_shapes(q.shape, k_pool.shape, block_tables.shape, ctx_lens.shape,
+                           q_start.shape)
+    nb, hkv, bs, d = k_pool.shape
+    B = ctx_lens.shape[0]
+    if max_q_len is None:
+        max_q_len = int((q_start[1:] - q_start[:-1]).max().item()) if B else 0
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    if out is None:
+        out = torch.zeros_like(q)
+    check(lib().rkv_prefill_attention_q(
+        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
+        ctx_lens.data_ptr(), B, q.shape[1], hkv, d, bs, nb, max_q_len, float(scale), code,
+        _stream(q)))
+    return out
+
+
+# ---- rotary positions ----------------------------------------------------------
+
+_ROPE = {None: _lib.RKV_ROPE_PLAIN, "linear": _lib.RKV_ROPE_LINEAR, "base": _lib.RKV_ROPE_BASE,
+         "parts": _lib.RKV_ROPE_PARTS, "bands": _lib.RKV_ROPE_BANDS}
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str | None = None,
+                     factor: float = 1.0, original_context: int = 0, low: float = 1.0,
+                     high: float = 32.0, device=None) -> tuple[torch.Tensor, float]:
+    """The table and magnitude that rope and rope_append take: float64
+    [rotary_dim / 2] on the device, and a float.  scaling: None, 'linear',
+    'base', 'parts' or 'bands' (rkv_rope_frequencies says what each does)."""
+    if scaling not in _ROPE:
+        raise ValueError(f"scaling {scaling!r}: want one of {list(_ROPE)}")
+    out = torch.empty(max(rotary_dim // 2, 0), dtype=torch.float64)
+    magnitude = torch.empty(1, dtype=torch.float32)
+    check(lib().rkv_rope_frequencies(out.data_ptr(), magnitude.data_ptr(), rotary_dim,
+                                     float(base), _ROPE[scaling], float(factor),
+                                     original_context, float(low), float(high)))
+    return out.to(device if device is not None else "cuda"), float(magnitude)
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """fp32 rows [T, H, D] whose elements are contiguous (a slice of a fused
+    projection's output is fine)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be {torch.float32}, got {t.dtype}")
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous rows")
+    return t
+
+
+def _rope_shapes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> None:
+    _dev(positions, "positions", torch.int32), _dev(inv_freq, "inv_freq", torch.float64)
+    if positions.shape != (x.shape[0],):
+        raise ValueError(f"{tuple(positions.shape)} positions for {x.shape[0]} tokens")
+    if inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > x.shape[2]:
+        raise ValueError("inv_freq must be [rotary_dim / 2] with rotary_dim <= head_dim")
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+         interleaved: bool = False, magnitude: float = 1.0,
+         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions: rows x [T, H, D] fp32 turned by positions [T] (int32)
+    times inv_freq (float64 [rotary_dim / 2], rope_frequencies).  The rotated
+    dims are the first rotary_dim, as pairs (i, i + rotary_dim / 2), or (2 i,
+    2 i + 1) with interleaved.  out may be x."""
+    _rows(x, "x")
+    _rope_shapes(x, positions, inv_freq)
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    elif _rows(out, "out").shape != x.shape:
+        raise ValueError("out must have x's shape")
+    t, h, d = x.shape
+    check(lib().rkv_rope(out.data_ptr(), x.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+                         t, h, d, 2 * inv_freq.shape[0], out.stride(0), out.stride(1),
+                         x.stride(0), x.stride(1), int(interleaved), magnitude, _stream(x)))
+    return out
+
+
+def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                positions: torch.Tensor, inv_freq: torch.Tensor, k_pool: torch.Tensor,
+                v_pool: torch.Tensor, slot_mapping: torch.Tensor, *, k_scale=None, v_scale=None,
+                fmt: str | None = None, interleaved: bool = False, magnitude: float = 1.0,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """One layer's rotation and append in one launch: returns rope(q), and the
+    pools get what append (fp32 and bf16 pools) or append_q (fmt 'int8' or 'fp8',
+    with the scale pools) of rope(k_new) and v_new writes.  Shapes as append's and
+    rope's; out may be q."""
+    _rows(q, "q"), _rows(k_new, "k_new"), _rows(v_new, "v_new")
+    _rope_shapes(q, positions, inv_freq)
+    _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool")
+    _dev(slot_mapping, "slot_mapping", torch.int64)
+    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+        raise ValueError("k_pool and v_pool must be one layer's pools of one shape and type")
+    nb, hkv, bs, d = k_pool.shape
+    t, hq, dq = q.shape
+    if k_new.shape != (t, hkv, d) or v_new.shape != (t, hkv, d) or dq != d:
+        raise ValueError(f"q {tuple(q.shape)}, k_new {tuple(k_new.shape)}, v_new "
+                         f"{tuple(v_new.shape)} do not match pool {tuple(k_pool.shape)}")
+    if k_new.stride() != v_new.stride():
+        raise ValueError("k_new and v_new must have the same strides")
+    if slot_mapping.shape != (t,):
+        raise ValueError("slot_mapping must be [n_tokens]")
+    if fmt is None:
+        code, ks, vs = _dtype_code(k_pool), None, None
+    else:
+        code = _qcode(fmt)
+        _dev(k_pool, "k_pool", torch.uint8)
+        if k_scale is None or v_scale is None:
+            raise ValueError("1-byte pools need their scale pools")
+        _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    elif _rows(out, "out").shape != q.shape:
+        raise ValueError("out must have q's shape")
+    check(lib().rkv_rope_append(
+        out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks, vs, q.data_ptr(),
+        k_new.data_ptr(), v_new.data_ptr(), out.stride(0), out.stride(1), q.stride(0),
+        q.stride(1), k_new.stride(0), k_new.stride(1), positions.data_ptr(), inv_freq.data_ptr(),
+        slot_mapping.data_ptr(), t, hq, hkv, d, 2 * inv_freq.shape[0], int(interleaved),
+        magnitude, bs, nb, code, _stream(q)))
+    return out
+
+
+# ---- eviction by accumulated attention weight ------------------------------------
+
+def weights_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                            max_context: int) -> int:
+    return int(lib().rkv_decode_weights_workspace_bytes(num_seqs, num_q_heads, num_kv_heads,
+                                                        head_dim, max_context))
+
+
+def _pool_code(k_pool, v_pool, k_scale, v_scale, fmt):
+    """(dtype code, k_scale pointer, v_scale pointer) of pools of any format."""
+    if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+        raise ValueError("k_pool and v_pool must have one shape and type")
+    if fmt is None:
+        return _dtype_code(k_pool), None, None
+    code = _anycode(fmt)
+    _dev(k_pool, "k_pool", torch.uint8)
+    if k_scale is None or v_scale is None:
+        raise ValueError("1-byte pools need their scale pools")
+    _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
+    return code, k_scale.data_ptr(), v_scale.data_ptr()
+
+
+def decode_attention_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                             weights: torch.Tensor, block_tables: torch.Tensor,
+                             ctx_lens: torch.Tensor, scale: float | None = None, *,
+                             k_scale=None, v_scale=None, fmt: str | None = None,
+                             max_context: int | None = None, out: torch.Tensor | None = None,
+                             workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """decode_attention that also adds to weights (fp32 [num_blocks, Hkv, 16])
+    the softmax weight each cached row received, summed over its KV head's query
+    heads.  fmt None: fp32 or bf16 pools; else a 1-byte format with its scale
+    pools.  workspace: weights_workspace_bytes."""
+    _dev(q, "q", torch.float32), _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool")
+    _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
+    _dev(weights, "weights", torch.float32)
+    check_attention_shapes(q.shape, k_pool.shape, block_tables.shape, ctx_lens.shape)
+    if weights.shape != k_pool.shape[:3]:
+        raise ValueError("weights must be the pools' shape without head_dim")
+    code, ks, vs = _pool_code(k_pool, v_pool, k_scale, v_scale, fmt)
+    nb, hkv, bs, d = k_pool.shape
+    B, hq, _ = q.shape
+    mbs = block_tables.shape[1]
+    if max_context is None:
+        max_context = mbs * bs
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    if out is None:
+        out = torch.empty_like(q)
+    if workspace is None:  # a caller's is checked by the library
+        need = weights_workspace_bytes(B, hq, hkv, d, max_context)
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    check(lib().rkv_decode_attention_weights(
+        out.data_ptr(), weights.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks,
+        vs, block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, max_context,
+        float(scale), code, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        _stream(q)))
+    return out
+
+
+def evict_select(weights: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor,
+                 budget: int, *, sinks: int = 4, recent: int = 0, max_context: int | None = None,
+                 keep: torch.Tensor | None = None, new_lens: torch.Tensor | None = None):
+    """The positions each KV head keeps of every sequence: its first `sinks`, its
+    last `recent` and of the others the largest weights (ties to the lower
+    position), `budget` in all.  weights [num_blocks, Hkv, 16] or [n_layers, ..].
+    Returns (keep int32 [.., B, Hkv, budget], ascending, -1 behind the last;
+    new_lens int32 [B])."""
+    _dev(weights, "weights", torch.float32)
+    _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
+    if weights.dim() not in (3, 4) or block_tables.dim() != 2 or ctx_lens.dim() != 1 or \
+            block_tables.shape[0] != ctx_lens.shape[0]:
+        raise ValueError("weights [.., num_blocks, Hkv, 16], one table row and length a sequence")
+    n_layers = weights.shape[0] if weights.dim() == 4 else 1
+    nb, hkv, bs = weights.shape[-3:]
+    B, mbs = block_tables.shape
+    shape = (*weights.shape[:-3], B, hkv, budget)
+    if keep is None:
+        keep = torch.empty(shape, dtype=torch.int32, device=weights.device)
+    elif _dev(keep, "keep", torch.int32).shape != shape:
+        raise ValueError(f"keep must be {shape}")
+    if new_lens is None:
+        new_lens = torch.empty(B, dtype=torch.int32, device=weights.device)
+    elif _dev(new_lens, "new_lens", torch.int32).shape != (B,):
+        raise ValueError("new_lens must be [B]")
+    check(lib().rkv_evict_select(keep.data_ptr(), new_lens.data_ptr(), weights.data_ptr(),
+                                 nb * hkv * bs, block_tables.data_ptr(), mbs, ctx_lens.data_ptr(),
+                                 B, n_layers, hkv, bs, nb, budget, sinks, recent,
+                                 mbs * bs if max_context is None else max_context,
+                                 _stream(weights)))
+    return keep, new_lens
+
+
+def evict_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, keep: torch.Tensor,
+                  new_lens: torch.Tensor, src_tables: torch.Tensor, dst_tables: torch.Tensor, *,
+                  k_scale=None, v_scale=None, weights: torch.Tensor | None = None,
+                  fmt: str | None = None) -> None:
+    """Moves the kept rows (evict_select) of every sequence and layer to positions
+    0 .. new_lens[b]-1 of dst_tables (int32 [B, blocks]), with their scales and
+    sums.  No destination block may be a source of the call or stand twice; the
+    source blocks stay as they are for the caller to free."""
+    _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), _dev(keep, "keep", torch.int32)
+    _dev(new_lens, "new_lens", torch.int32), _dev(src_tables, "src_tables", torch.int32)
+    _dev(dst_tables, "dst_tables", torch.int32)
+    if k_pool.dim() not in (4, 5):
+        raise ValueError("pools must be [num_blocks, Hkv, 16, D] or [n_layers, ..]")
+    code, ks, vs = _pool_code(k_pool, v_pool, k_scale, v_scale, fmt)
+    nb, hkv, bs, d = k_pool.shape[-4:]
+    n_layers = k_pool.shape[0] if k_pool.dim() == 5 else 1
+    B = new_lens.shape[0]
+    if keep.dim() != k_pool.dim() - 1 or keep.shape[:-1] != (*k_pool.shape[:-4], B, hkv):
+        raise ValueError(f"keep shape {tuple(keep.shape)} does not match pool {tuple(k_pool.shape)}")
+    if src_tables.dim() != 2 or dst_tables.dim() != 2 or src_tables.shape[0] != B or \
+            dst_tables.shape[0] != B:
+        raise ValueError("one source and one destination table row per sequence")
+    if weights is not None and _dev(weights, "weights", torch.float32).shape != k_pool.shape[:-1]:
+        raise ValueError("weights must be the pools' shape without head_dim")
+    check(lib().rkv_evict_compact(
+        k_pool.data_ptr(), v_pool.data_ptr(), ks, vs,
+        weights.data_ptr() if weights is not None else None, nb * hkv * bs * d, nb * hkv * bs,
+        keep.data_ptr(), new_lens.data_ptr(), keep.shape[-1], src_tables.data_ptr(),
+        src_tables.shape[1], dst_tables.data_ptr(), dst_tables.shape[1], B, n_layers, hkv, d, bs,
+        nb, code, _stream(k_pool)))
 
 
 class DeviceBlockManager:
@@ -555,4 +896,6 @@ class DeviceBlockManager:
 __all__ = ["append", "gather", "copy_blocks", "decode_attention", "prefill_attention",
            "append_q", "gather_q", "decode_attention_q", "workspace_bytes",
            "DeviceBlockManager", "_lib", "partition_size_for", "decode_attention_append",
-           "decode_attention_append_q"]
+           "decode_attention_append_q", "append_block_q", "prefill_attention_q",
+           "rope_frequencies", "rope", "rope_append", "weights_workspace_bytes",
+           "decode_attention_weights", "evict_select", "evict_compact"]

@@ -358,6 +358,82 @@ def argmax(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be {torch.float32}, got {t.dtype}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be [rows, vocab] with contiguous rows")
+    return t
+
+
+def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
+                   history_start: torch.Tensor | None = None,
+                   prompt_lens: torch.Tensor | None = None,
+                   repetition: torch.Tensor | None = None,
+                   frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                   bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   bias_start: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None, pick: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None):
+    """Penalties, biases and masks on logits [rows, vocab] fp32, and the greedy
+    pick: (processed logits, pick int32 [rows]).  Row r's token ids are
+    history[history_start[r] : history_start[r+1]] (int32), the first
+    prompt_lens[r] of them its prompt; repetition, frequency and presence are
+    fp32 [rows]; bias_ids / bias are the rows' (token, value) entries between
+    the offsets bias_start; allowed holds a bit a token in int32 words
+    [rows, >= ceil(vocab / 32)].  The pick is argmax's, -1 where a row has
+    nothing left.  out may be logits.  rkv_process_logits has the formulas."""
+    _matrix(logits, "logits")
+    rows, n = logits.shape
+    dev = logits.device
+
+    def ptr(t, name, dtype, shape):
+        if t is None:
+            return None
+        if _dev(t, name, dtype).shape != shape:
+            raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+        return t.data_ptr()
+
+    per, ends = (rows,), (rows + 1,)
+    if allowed is not None and (_dev(allowed, "allowed", torch.int32).dim() != 2 or
+                                allowed.shape[0] != rows or allowed.shape[1] < -(-n // 32)):
+        raise ValueError(f"allowed must be [{rows}, {-(-n // 32)}] words or wider")
+    if bias_ids is not None and (bias is None or bias_start is None or
+                                 bias_ids.shape != bias.shape or bias_ids.dim() != 1):
+        raise ValueError("bias_ids needs bias of the same length and bias_start")
+    if history is not None and _dev(history, "history", torch.int32).dim() != 1:
+        raise ValueError("history must be one row of token ids")
+    if out is None:
+        out = torch.empty((rows, n), dtype=torch.float32, device=dev)
+    elif _matrix(out, "out").shape != logits.shape:
+        raise ValueError("out must have the logits' shape")
+    if pick is None:
+        pick = torch.empty(rows, dtype=torch.int32, device=dev)
+    if workspace is None:
+        need = lib().rkv_process_logits_workspace_bytes(rows, n)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    check(lib().rkv_process_logits(
+        out.data_ptr(), out.stride(0), ptr(pick, "pick", torch.int32, per), logits.data_ptr(),
+        logits.stride(0), rows, n, None if history is None else history.data_ptr(),
+        ptr(history_start, "history_start", torch.int32, ends),
+        ptr(prompt_lens, "prompt_lens", torch.int32, per),
+        ptr(repetition, "repetition", torch.float32, per),
+        ptr(frequency, "frequency", torch.float32, per),
+        ptr(presence, "presence", torch.float32, per),
+        None if bias_ids is None else _dev(bias_ids, "bias_ids", torch.int32).data_ptr(),
+        None if bias_ids is None else _dev(bias, "bias", torch.float32).data_ptr(),
+        None if bias_ids is None else ptr(bias_start, "bias_start", torch.int32, ends),
+        None if allowed is None else allowed.data_ptr(),
+        0 if allowed is None else allowed.shape[1],
+        None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel() * workspace.element_size(),
+        _stream(logits)))
+    return out, pick
+
+
 def embed(table: torch.Tensor, ids: torch.Tensor, pe: torch.Tensor | None = None,
           positions: torch.Tensor | None = None) -> torch.Tensor:
     _dev(table, "table", torch.float32), _dev(ids, "ids", torch.int32)
@@ -372,4 +448,4 @@ def embed(table: torch.Tensor, ids: torch.Tensor, pe: torch.Tensor | None = None
 
 __all__ = ["DecoderConfig", "CONFIG0", "config", "param_count", "init_params", "rng_raw",
            "fill_normal", "Decoder", "linear", "layer_norm", "qkv_append", "gelu", "add", "argmax",
-           "embed", "mul_scalar", "softmax_dim", "matmul", "transpose"]
+           "process_logits", "embed", "mul_scalar", "softmax_dim", "matmul", "transpose"]
