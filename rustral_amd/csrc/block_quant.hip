@@ -90,8 +90,7 @@ __global__ __launch_bounds__(256) void append_block_q_kernel(
   for (int i = 0; i < NP; ++i) {
     const int r = RPP * i + sub;
     if (r >= lo && r < hi)
-      dst[r * U + c] = tile_byte<DT>(x[i].x, s, inv) | tile_byte<DT>(x[i].y, s, inv) << 8 |
-                       tile_byte<DT>(x[i].z, s, inv) << 16 | tile_byte<DT>(x[i].w, s, inv) << 24;
+      dst[r * U + c] = tile_word<DT>(x[i], s, inv);
   }
   if (lane == 0 && (lo == 0 || grew)) *sp = s;
 }

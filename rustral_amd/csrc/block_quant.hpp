@@ -4,7 +4,7 @@
 //
 // Bytes are the exactly rounded quotients x / scale and byte * old / scale
 // (nearest, ties to even), so they do not depend on how a quotient was
-// approximated: an int8 product with the reciprocal is within 2^-15 of the
+// approximated: an int8 product with the reciprocal or the ratio is within 2^-15 of the
 // quotient (|quotient| <= 127, three roundings of 2^-24), and where it falls
 // that near to the middle between two integers the remainder is formed in 64
 // bits, exactly (24 and 31 bit factors), and decides.
@@ -39,52 +39,100 @@ __device__ __forceinline__ float tile_scale(float amax) {
   }
 }
 
-// r, the rounding of y, corrected to that of the exact num / den (y is within
-// 2^-15 of it).
-__device__ __forceinline__ float exact_round(float y, double num, double den) {
-  float r = fminf(fmaxf(rintf(y), -127.0f), 127.0f);
-  if (fabsf(fabsf(y - r) - 0.5f) < 1e-4f) {
-    const double e = fma(-(double)r, den, num), h = 0.5 * den;
-    const bool odd = ((int)r & 1) != 0;
-    if (e > h || (e == h && odd)) r += 1.0f;
-    if (e < -h || (e == -h && odd)) r -= 1.0f;
-    r = fminf(fmaxf(r, -127.0f), 127.0f);
-  }
+// Whether y may be on the wrong side of the middle between two integers (y is within
+// 2^-15 of the quotient it stands for; r = rintf(y)).
+__device__ __forceinline__ bool near_middle(float y, float r) { return fabsf(y - r) > 0.4999f; }
+
+// r, the rounding of a quotient's approximation, corrected to that of num / den.
+__device__ __forceinline__ float exact_round(float r, double num, double den) {
+  const double e = fma(-(double)r, den, num), h = 0.5 * den;
+  const bool odd = ((int)r & 1) != 0;
+  if (e > h || (e == h && odd)) r += 1.0f;
+  if (e < -h || (e == -h && odd)) r -= 1.0f;
   return r;
 }
 
-// Byte of x under scale s (inv = 1 / s, or 0 for s = 0).
+// Four floats of at most 448 in magnitude as e4m3 bytes, round to nearest even:
+// v_cvt_pk_fp8_f32, whose bytes are e4m3_from_f32's (checked on the GPU).  A NaN
+// loses its sign on the way: its byte is taken from `nan`.
+__device__ __forceinline__ uint32_t pack_e4m3x4(const float (&v)[4], uint32_t nan) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+  if (!(v[0] == v[0] && v[1] == v[1] && v[2] == v[2] && v[3] == v[3])) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t m = 0xffu << (8 * e);
+      if (v[e] != v[e]) w = (int)(((uint32_t)w & ~m) | (nan & m));
+    }
+  }
+  return (uint32_t)w;
+}
+
+// The bytes of four values under scale s (inv = 1 / s, or 0 for s = 0).
 template <int DT>
-__device__ __forceinline__ uint32_t tile_byte(float x, float s, float inv) {
+__device__ __forceinline__ uint32_t tile_word(const float4& x, float s, float inv) {
+  const float v[4] = {x.x, x.y, x.z, x.w};
   if constexpr (DT == RKV_I8_BLOCK) {
-    if (!(x == x) || s == 0.0f) return 0u;
-    return (uint32_t)(int)exact_round(x * inv, (double)x, (double)s) & 0xffu;
+    float r[4];
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = v[e] * inv;  // an infinity: clamped; a NaN (of x, or 0 times an infinity): 0
+      r[e] = rintf(y);
+      near = near || near_middle(y, r[e]);
+      r[e] = y == y ? fminf(fmaxf(r[e], -127.0f), 127.0f) : 0.0f;
+    }
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (fabsf(v[e]) < INFINITY) r[e] = exact_round(r[e], (double)v[e], (double)s);
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w |= ((uint32_t)(int)r[e] & 0xffu) << (8 * e);
+    return w;
   } else {
-    if (x == x && s == 0.0f) return 0u;
-    return e4m3_from_f32(x * inv);
+    float y[4];
+    uint32_t nan = 0x7f7f7f7fu;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      nan |= (__float_as_uint(v[e]) >> 31) << (8 * e + 7);
+      const float c = s > 0.0f ? __builtin_amdgcn_fmed3f(v[e] * inv, -448.0f, 448.0f) : 0.0f;
+      y[e] = v[e] == v[e] ? c : v[e];
+    }
+    return pack_e4m3x4(y, nan);
   }
 }
 
-// Byte b of a tile of scale s_old under scale s >= s_old (ratio = s_old / s).
-template <int DT>
-__device__ __forceinline__ uint32_t tile_rebyte(uint32_t b, float s_old, float s, float ratio) {
-  if constexpr (DT == RKV_I8_BLOCK) {
-    const float v = (float)(int8_t)b;
-    if (s == 0.0f) return 0u;
-    return (uint32_t)(int)exact_round(v * ratio, (double)v * (double)s_old, (double)s) & 0xffu;
-  } else {
-    return e4m3_from_f32(f32_from_e4m3((uint8_t)b) * ratio);
-  }
-}
-
-// The four bytes of a word so treated.
+// The four bytes of a word of a tile of scale s_old brought to scale s >= s_old,
+// s > 0 (ratio = s_old / s).
 template <int DT>
 __device__ __forceinline__ uint32_t tile_reword(uint32_t w, float s_old, float s, float ratio) {
-  uint32_t o = 0;
+  if constexpr (DT == RKV_I8_BLOCK) {
+    float r[4];
+    bool near = false;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    o |= tile_rebyte<DT>((w >> (8 * e)) & 0xffu, s_old, s, ratio) << (8 * e);
-  return o;
+    for (int e = 0; e < 4; ++e) {
+      const float y = (float)((int32_t)(w << (24 - 8 * e)) >> 24) * ratio;
+      r[e] = rintf(y);
+      near = near || near_middle(y, r[e]);
+    }
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[e] = exact_round(r[e], (double)((int32_t)(w << (24 - 8 * e)) >> 24) * (double)s_old,
+                           (double)s);
+    }
+    uint32_t o = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o |= ((uint32_t)(int)r[e] & 0xffu) << (8 * e);
+    return o;
+  } else {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    const float v[4] = {lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio};
+    return pack_e4m3x4(v, w);
+  }
 }
 
 }  // namespace rkv

@@ -246,6 +246,19 @@ __device__ __forceinline__ float lo_col(float x) {
   return dpp<CTRL>(x);
 }
 
+// The sum of a product's three columns l, l + G and l + 2 G for the lanes l % 16 < G
+// <= 4 (other lanes: any value).  row_shl:n hands lane l the value of lane l + n of
+// its 16-lane row, 0 past the row's end, as an operand of the addition itself.
+template <int G>
+__device__ __forceinline__ float three_cols(float x) {
+  auto from = [](float v, auto n) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(
+        0, __float_as_int(v), 0x100 + decltype(n)::value, 0xf, 0xf, true));
+  };
+  return (x + from(x, std::integral_constant<int, G>{})) +
+         from(x, std::integral_constant<int, 2 * G>{});
+}
+
 // ---- streaming variant ---------------------------------------------------------
 // SPLIT 64-lane waves own one (partition, KV head, sequence) item; a
 // partition is SPLIT * tw blocks (tw = tiles_per_wave <= NTW = NTILE / SPLIT,
@@ -303,10 +316,19 @@ __device__ __forceinline__ float lo_col(float x) {
 // (m, l), also a sequence's only one.
 // Formats with one scale a tile (RKV_I8_BLOCK, RKV_FP8_BLOCK) run the row-scaled
 // formats' code with the tile's scale in the place of its rows'.
+template <int G, int FORMAT, DecodeMode MODE>
+constexpr int waves_per_simd() {
+  if (G >= 8) return 2;
+  // the builds with three terms hold the same four workgroups as the others when
+  // the scheduler is kept to 128 registers
+  const bool three = FORMAT == RKV_FP8_BLOCK || (MODE == kScores && FORMAT != RKV_F32);
+  return three ? 4 : RKV_DECODE_WAVES_PER_SIMD;
+}
+
 template <typename T, int D, int G, int BS, int NTILE, int R, int SPLIT, int FORMAT,
           DecodeMode MODE = kAttend>
 __global__ __launch_bounds__(64 * SPLIT)
-__attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) void decode_stream_kernel(
+__attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void decode_stream_kernel(
     float* __restrict__ out, float* __restrict__ part_acc, float* __restrict__ part_ml,
     const float* __restrict__ q, const void* __restrict__ k_pool_,
     const void* __restrict__ v_pool_, const float* __restrict__ k_scale,
@@ -366,6 +388,12 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
   }
   // 1-byte pools (QNT): bytes plus one fp32 scale per (token, KV head) row.
   constexpr bool QNT = FMT == RKV_I8 || FMT == RKV_FP8;
+  // bf16 terms of a q element or a softmax weight on the matrix cores: hi + lo (16
+  // significant bits), and in the builds that came with the block-scaled formats
+  // and the scores a third (24 bits, as many as fp32: 3.6e-6 off the exact rows
+  // with two, about 4e-7 with three).  The operand has 16 rows, so the third term
+  // of up to 5 heads takes rows that were zero; the earlier builds keep their bits.
+  constexpr int TERMS = (TSC || MODE == kScores) && G <= 4 ? 3 : 2;
   static_assert(QNT == (sizeof(T) == 1), "1-byte element type iff a 1-byte format");
   constexpr bool MFMA = (sizeof(T) == 2 || QNT) && 2 * G <= 16;
   // PV on the matrix cores as well (bf16 and 1-byte pools):
@@ -433,7 +461,7 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
       qv[e + 0] = x.x; qv[e + 1] = x.y; qv[e + 2] = x.z; qv[e + 3] = x.w;
     }
   } else if constexpr (MFMA) {
-    const int qrow = kt < G ? kt : (kt < 2 * G ? kt - G : 0);
+    const int qrow = kt < TERMS * G ? kt % G : 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d0 = QNT ? (D / 4) * kq + 8 * c : 32 * c + 8 * kq;
@@ -689,13 +717,41 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
       for (int e = 0; e < 4; ++e) {
         const float x = qv[c * 8 + 2 * e], y = qv[c * 8 + 2 * e + 1];
         const uint32_t hi = cvt_bf16x2(x, y);
-        const uint32_t lo =
-            cvt_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+        const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xffff0000u);
+        const uint32_t lo = cvt_bf16x2(rx, ry);
         h[e] = kt < G ? hi : (kt < 2 * G ? lo : 0u);
+        if constexpr (TERMS == 3) {
+          const uint32_t last = cvt_bf16x2(rx - __uint_as_float(lo << 16),
+                                           ry - __uint_as_float(lo & 0xffff0000u));
+          h[e] = kt >= 2 * G && kt < 3 * G ? last : h[e];
+        }
       }
       qa[c] = make_uint4(h[0], h[1], h[2], h[3]);
     }
   }
+
+  // kScores: this slice's scores, G to a position, contiguous over the wave.  Where
+  // the buffer keeps them (MFMA builds) they are stored behind the last V tile's
+  // request: loads and stores share one in-order counter, so a tile requested
+  // behind the stores would wait for them.
+  auto put_scores = [&]() __attribute__((always_inline)) {
+    float* sp = scores + (((int64_t)b * num_kv_heads + kh) * ((int64_t)max_parts * P) + tok0) * G;
+    const int live = tw * BS < L - tok0 ? tw * BS : L - tok0;  // may be <= 0
+#pragma unroll
+    for (int x = lane; x < NTW * BS; x += 64)
+      if (x < live) {
+        if constexpr (G % 4 == 0) {
+#pragma unroll
+          for (int g = 0; g < G; g += 4)
+            *reinterpret_cast<float4*>(sp + x * G + g) =
+                *reinterpret_cast<const float4*>(s_p + x * G + g);
+        } else if constexpr (G == 2) {
+          *reinterpret_cast<float2*>(sp + x * 2) = *reinterpret_cast<const float2*>(s_p + x * 2);
+        } else {
+          sp[x] = s_p[x];
+        }
+      }
+  };
 
   // The 2*NTW steps are instantiated one by one (static_for) so that every
   // ring slot is a fixed set of registers.
@@ -717,6 +773,7 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
       }
     };
     constexpr bool staged = t < NTW ? KLDS : MPV;
+    if constexpr (MODE == kScores && MPV && t == (NT - R > NTW ? NT - R : NTW)) put_scores();
     if constexpr (t < NTW) {
       // ---- QK^T for the 16 tokens of tile i ----
       if constexpr (MFMA) {
@@ -782,18 +839,26 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
         if constexpr (I8QK) {
           if (kq < G) s_p[tp * G + kq] = valid ? sacc[0] * qs : -INFINITY;
         } else if constexpr (G == 1) {
-          if (kq == 0) s_p[tp] = valid ? (sacc[0] + sacc[1]) * qs : -INFINITY;
+          float dot = sacc[0] + sacc[1];
+          if constexpr (TERMS == 3) dot += sacc[2];
+          if (kq == 0) s_p[tp] = valid ? dot * qs : -INFINITY;
         } else if constexpr (G == 2) {
+          float d0 = sacc[0] + sacc[2], d1 = sacc[1] + sacc[3];
+          // rows 4 and 5, the third terms, are 16 lanes on (rows 6 and 7 are zero)
+          if constexpr (TERMS == 3) d0 = pair16_sum(d0), d1 = pair16_sum(d1);
           if (kq == 0) {
-            s_p[tp * 2 + 0] = valid ? (sacc[0] + sacc[2]) * qs : -INFINITY;
-            s_p[tp * 2 + 1] = valid ? (sacc[1] + sacc[3]) * qs : -INFINITY;
+            s_p[tp * 2 + 0] = valid ? d0 * qs : -INFINITY;
+            s_p[tp * 2 + 1] = valid ? d1 * qs : -INFINITY;
           }
         } else {
           constexpr int XOR = G == 4 ? 16 : 32;  // lanes between hi and lo rows
           float sc[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            sc[r] = (XOR == 16 ? pair16_sum(sacc[r]) : pair32_sum(sacc[r])) * qs;
+          for (int r = 0; r < 4; ++r) {
+            const float d = XOR == 16 ? pair16_sum(sacc[r]) : pair32_sum(sacc[r]);
+            // rows 8 .. 11, the third terms, are 32 lanes on (12 .. 15 are zero)
+            sc[r] = (TERMS == 3 ? pair32_sum(d) : d) * qs;
+          }
           if (lane < XOR) {  // lanes kq * 16 + kt hold heads 4 kq .. 4 kq + 3
             *reinterpret_cast<float4*>(&s_p[tp * G + 4 * kq]) =
                 valid ? make_float4(sc[0], sc[1], sc[2], sc[3])
@@ -826,25 +891,8 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // LDS writes above ...
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");  // ... before the reads below
-        if constexpr (MODE == kScores) {
-          // this slice's scores, G to a position: contiguous over the wave
-          float* sp = scores + (((int64_t)b * num_kv_heads + kh) * ((int64_t)max_parts * P) + tok0) * G;
-          const int live = tw * BS < L - tok0 ? tw * BS : L - tok0;  // may be <= 0
-#pragma unroll
-          for (int x = lane; x < NTW * BS; x += 64)
-            if (x < live) {
-              if constexpr (G % 4 == 0) {
-#pragma unroll
-                for (int g = 0; g < G; g += 4)
-                  *reinterpret_cast<float4*>(sp + x * G + g) =
-                      *reinterpret_cast<const float4*>(s_p + x * G + g);
-              } else if constexpr (G == 2) {
-                *reinterpret_cast<float2*>(sp + x * 2) = *reinterpret_cast<const float2*>(s_p + x * 2);
-              } else {
-                sp[x] = s_p[x];
-              }
-            }
-        }
+        // fp32 pools overwrite the scores with the weights next
+        if constexpr (MODE == kScores && !MPV) put_scores();
 #pragma unroll
         for (int g = 0; g < G; ++g) m[g] = -INFINITY;
 #pragma unroll
@@ -965,15 +1013,23 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");  // ... before the reads below
         // B = P^T (16 x 16 x 16): k-slot 4 kq + e holds key 4 kq + e of the
         // tile, column kt
-        const int pc = kt < G ? kt : (kt < 2 * G ? kt - G : 0);
+        const int pc = kt < TERMS * G ? kt % G : 0;
         const float4 p4 = *reinterpret_cast<const float4*>(&s_pq[w][pc * NK + i * BS + 4 * kq]);
         const uint32_t h0 = cvt_bf16x2(p4.x, p4.y), h1 = cvt_bf16x2(p4.z, p4.w);
-        const uint32_t l0 =
-            cvt_bf16x2(p4.x - __uint_as_float(h0 << 16), p4.y - __uint_as_float(h0 & 0xffff0000u));
-        const uint32_t l1 =
-            cvt_bf16x2(p4.z - __uint_as_float(h1 << 16), p4.w - __uint_as_float(h1 & 0xffff0000u));
-        const uint2 pb = kt < G ? make_uint2(h0, h1)
-                                : (kt < 2 * G ? make_uint2(l0, l1) : make_uint2(0u, 0u));
+        const float rx = p4.x - __uint_as_float(h0 << 16);
+        const float ry = p4.y - __uint_as_float(h0 & 0xffff0000u);
+        const float rz = p4.z - __uint_as_float(h1 << 16);
+        const float rw = p4.w - __uint_as_float(h1 & 0xffff0000u);
+        const uint32_t l0 = cvt_bf16x2(rx, ry), l1 = cvt_bf16x2(rz, rw);
+        uint2 pb = kt < G ? make_uint2(h0, h1)
+                          : (kt < 2 * G ? make_uint2(l0, l1) : make_uint2(0u, 0u));
+        if constexpr (TERMS == 3) {
+          const uint32_t t0 = cvt_bf16x2(rx - __uint_as_float(l0 << 16),
+                                         ry - __uint_as_float(l0 & 0xffff0000u));
+          const uint32_t t1 = cvt_bf16x2(rz - __uint_as_float(l1 << 16),
+                                         rw - __uint_as_float(l1 & 0xffff0000u));
+          if (kt >= 2 * G && kt < 3 * G) pb = make_uint2(t0, t1);
+        }
         // A = V^T: this lane's read address is key 4 kq + (kt >> 2), dims
         // 16 c + 4 (kt & 3) .. + 3
         const uint8_t* va = vb + (4 * kq + (kt >> 2)) * VROW + 8 * (kt & 3);
@@ -1014,7 +1070,7 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");  // ... before the reads below
         // B = P^T: lane (kq, kt) holds keys 8 kq .. + 7 of the pair, column kt
-        const int pc = kt < G ? kt : (kt < 2 * G ? kt - G : 0);
+        const int pc = kt < TERMS * G ? kt % G : 0;
         const float* pp = &s_pq[w][pc * NK + (i - 1) * BS + 8 * kq];
         const float4 p0 = reinterpret_cast<const float4*>(pp)[0];
         const float4 p1 = reinterpret_cast<const float4*>(pp)[1];
@@ -1024,9 +1080,15 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
         for (int e = 0; e < 4; ++e) {
           const float x = pv8[2 * e], y = pv8[2 * e + 1];
           const uint32_t hi = cvt_bf16x2(x, y);  // round to nearest even (p is finite)
-          const uint32_t lo =
-              cvt_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+          const float rx = x - __uint_as_float(hi << 16);
+          const float ry = y - __uint_as_float(hi & 0xffff0000u);
+          const uint32_t lo = cvt_bf16x2(rx, ry);
           pw[e] = kt < G ? hi : (kt < 2 * G ? lo : 0u);
+          if constexpr (TERMS == 3) {
+            const uint32_t last = cvt_bf16x2(rx - __uint_as_float(lo << 16),
+                                             ry - __uint_as_float(lo & 0xffff0000u));
+            pw[e] = kt >= 2 * G && kt < 3 * G ? last : pw[e];
+          }
         }
         const uint4 pb = make_uint4(pw[0], pw[1], pw[2], pw[3]);
         // A = V^T, 16 dims per MFMA: this lane's read address is key
@@ -1079,7 +1141,8 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
   });
 
   // MFMA PV: lane (kq, kt) holds O^T[dim 16 c + 4 kq + r][column kt]; head
-  // g's sum is column g (hi) plus column G + g (lo): lanes kt < G take it.
+  // g's sum is column g (hi) plus column G + g (lo), and 2 G + g with three terms:
+  // lanes kt < G take it.
   // I8PV: lane (kq, kt) holds head kq's sums for dims 16 c + kt.
   f32x4_t hv[MPV && !I8PV ? D / 16 : 1];
   float iv[I8PV ? D / 16 : 1];
@@ -1093,7 +1156,10 @@ __attribute__((amdgpu_waves_per_eu(G >= 8 ? 2 : RKV_DECODE_WAVES_PER_SIMD))) voi
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) hv[c][r] = ov[c][r] + lo_col<G>(ov[c][r]);
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (TERMS == 3) hv[c][r] = three_cols<G>(ov[c][r]);
+        else hv[c][r] = ov[c][r] + lo_col<G>(ov[c][r]);
+      }
   } else {
     // sum over the TPL token rows, then lanes of row 0 hold the result
 #pragma unroll
@@ -1277,10 +1343,10 @@ Launch make_launch(DecodeMode mode) {
     if constexpr (FMT == RKV_BF16 || FMT == RKV_I8 || FMT == RKV_FP8)
       l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, R, SPLIT, FMT, kAppend>;
   } else if (mode == kScores) {
-    // the 8-wave builds and the ones between the smallest and the small
-    // partition have no score form (pick_p asks for none)
-    if constexpr (SPLIT == split_of<T>() && (NTILE == kShortP / kBS || NTILE == kSmallP / kBS ||
-                                             NTILE == part_of<T>() / kBS))
+    // no score form between the smallest and the small partition (pick_p asks for
+    // none)
+    if constexpr (SPLIT != split_of<T>() || NTILE == kShortP / kBS || NTILE == kSmallP / kBS ||
+                  NTILE == part_of<T>() / kBS)
       l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, R, SPLIT, FMT, kScores>;
   } else {
     l.kernel = &decode_stream_kernel<T, D, G, kBS, NTILE, R, SPLIT, FMT>;

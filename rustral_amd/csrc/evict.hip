@@ -4,6 +4,8 @@
 // rkv_decode_attention_weights (paged_decode.hip).
 #include "block_quant.hpp"
 
+#include <type_traits>
+
 namespace rkv {
 namespace {
 
@@ -13,17 +15,23 @@ constexpr int kBS = 16;
 // One workgroup per (layer, sequence, KV head).  Every position becomes a 32-bit
 // key that orders like (class, weight): 0 absent, 1 a NaN sum, then the sums in
 // float order, all ones the first and last positions, which are always kept.
-// The n-th largest key is built bit by bit from the top: a bit stays set if at
-// least n keys reach the candidate, so 32 counts at most, fewer when a candidate
-// is reached by exactly n.  A count is a ballot per four keys and a sum over the
-// waves in LDS; the keys stay in registers (J groups of four a thread), or are
-// read again for each count where a context is longer than the registers hold
-// (J = 0).
-// Positions are then taken in order: a key above the threshold is kept, one that
-// equals it while the count lasts, so ties go to the lower position.  With both
-// counts in one prefix sum, the place of a position is
-//   (above before it) + min(equal before it, equal wanted).
-// Thread t of NT holds positions 4 (t + NT j) .. + 3, a float4 of one block.
+// The n-th largest key is found by digits of 11, 11 and 10 bits from the top: a
+// histogram in LDS of the keys that share the digits found so far, a sum over its
+// bins from the top, and the bin where it passes what is still wanted.  Counts are
+// integers, so their order does not matter.  It ends early where a bin is wanted
+// whole.  Keys are formed once and kept in LDS for up to kKeysMax positions (KEYS);
+// a longer context is read again by each of the passes.
+// A wave owns a contiguous run of positions, so the kept ones' places need one
+// exchange of the waves' totals; inside a wave they come from ballots: with the
+// keys above the threshold and those that equal it counted apart, the place of a
+// position is  (above before it) + min(equal before it, equal wanted),  so ties go
+// to the lower position.
+// Lane l of a step holds 4 positions, a float4 of one block.  The loops stay rolled:
+// a grid of few workgroups runs each instruction about once.
+// us for 8 layers x 16 sequences of U[1500, 4096] / 2 layers x 1 of 32,768, 8 KV
+// heads: 29.5 / 66 with keys in registers (unrolled) and 32 counts of the keys above
+// a candidate; 29.6 / 44.7 with keys in LDS and counts at candidates on a line
+// between the last two; 18.1 / 30.1 with the digits.
 
 __device__ __forceinline__ uint32_t weight_key(float w) {
   const uint32_t u = __float_as_uint(w + 0.0f);  // -0 and +0 are one weight
@@ -31,7 +39,24 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return w == w ? k : 1u;
 }
 
-template <int NT, int J>
+constexpr uint32_t kHeld = 0xffffffffu;
+constexpr int kBins = 2048;
+constexpr int kKeysMax = 32768;  // positions whose keys fit in LDS beside the bins
+
+// Inclusive prefix sum over the wave: row_shr 1, 2, 4, 8 inside each 16-lane row
+// (0 past its start), then the last lane of row 0 added to row 1 and of row 2 to row
+// 3 (row_bcast:15), and of row 1 to rows 2 and 3 (row_bcast:31).
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
+template <int NT, bool KEYS>
 __global__ __launch_bounds__(NT) void evict_select_kernel(
     int32_t* __restrict__ keep, int32_t* __restrict__ new_lens,
     const float* __restrict__ weights, int64_t weights_layer_stride,
@@ -39,8 +64,12 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
     const int32_t* __restrict__ ctx_lens, int num_kv_heads, int64_t num_blocks, int budget,
     int sinks, int recent, int cap) {
   constexpr int NW = NT / 64;
-  constexpr int JR = J ? J : 1;
-  __shared__ int s_cnt[2][NW];
+  constexpr int BPT = kBins / NT;  // bins a thread
+  extern __shared__ __align__(16) uint4 s_key[];  // KEYS: four positions each
+  __shared__ __align__(16) uint32_t s_bin[kBins];
+  __shared__ uint32_t s_sum[NW];
+  __shared__ uint32_t s_found[3];  // the bin, its count, the count above it
+  __shared__ int2 s_tot[NW];
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -49,124 +78,189 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
   const int32_t* __restrict__ tab = block_tables + (int64_t)b * max_blocks_per_seq;
   const float* __restrict__ wl = weights + layer * weights_layer_stride;
   const int groups = (L + 3) / 4;
-  const int nj = (groups + NT - 1) / NT;
+  const int steps = ((groups + 63) / 64 + NW - 1) / NW;  // of a wave
+  const int g0 = w * steps * 64 + lane;                  // this lane's group of step 0
 
-  auto load_keys = [&](int j, uint32_t (&k)[4]) {
-    const int g = tid + NT * j, p = 4 * g;
-    k[0] = k[1] = k[2] = k[3] = 0u;
+  auto form = [&](int g) __attribute__((always_inline)) {
+    uint4 k = make_uint4(0u, 0u, 0u, 0u);
+    const int p = 4 * g;
     if (g < groups) {
       const int32_t blk = tab[p / kBS];
       if (blk >= 0 && blk < num_blocks) {
         const float4 v = *reinterpret_cast<const float4*>(
             wl + ((int64_t)blk * num_kv_heads + h) * kBS + p % kBS);
-        const float vv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int q = p + e;
+        auto one = [&](float x, int q) -> uint32_t {
           const bool held = q < sinks || q >= L - recent;
-          k[e] = q < L ? (held ? 0xffffffffu : weight_key(vv[e])) : 0u;
-        }
+          return q < L ? (held ? kHeld : weight_key(x)) : 0u;
+        };
+        k = make_uint4(one(v.x, p), one(v.y, p + 1), one(v.z, p + 2), one(v.w, p + 3));
       }
     }
+    return k;
   };
-  uint32_t key[JR][4];
-  if constexpr (J > 0) {
-#pragma unroll
-    for (int j = 0; j < J; ++j) load_keys(j, key[j]);
+  // Keys of this lane's group of a step.  A lane reads back only what it wrote.
+  auto keys = [&](int j) __attribute__((always_inline)) {
+    const int g = g0 + 64 * j;
+    if constexpr (KEYS) return g < groups ? s_key[g] : make_uint4(0u, 0u, 0u, 0u);
+    else return form(g);
+  };
+  if constexpr (KEYS) {
+#pragma unroll 4
+    for (int j = 0; j < steps; ++j) {
+      const int g = g0 + 64 * j;
+      const uint4 k = form(g);
+      if (g < groups) s_key[g] = k;
+    }
   }
-  auto for_keys = [&](auto&& f) __attribute__((always_inline)) {
-    if constexpr (J > 0) {
+
+  // Histogram of digit (key >> shift) % bins over the non-zero keys whose bits above
+  // are `top` (at shift + digit bits), and the bin from the top where the count
+  // reaches `want`: s_found.  Returns the histogram's total.
+  auto digit = [&](int shift, int bits, uint32_t top, uint32_t want) __attribute__((always_inline)) {
+    const uint32_t mask = (1u << bits) - 1u;
 #pragma unroll
-      for (int j = 0; j < J; ++j) f(j, key[j]);
-    } else {
-      for (int j = 0; j < nj; ++j) {
-        uint32_t k[4];
-        load_keys(j, k);
-        f(j, k);
-      }
-    }
-  };
-  int buf = 0;
-  // Keys >= t in the workgroup, the same in every thread.
-  auto count = [&](uint32_t t) {
-    int c = 0;
-    for_keys([&](int, const uint32_t (&k)[4]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c += __popcll(__builtin_amdgcn_ballot_w64(k[e] >= t));
-    });
-    if (lane == 0) s_cnt[buf][w] = c;
+    for (int i = 0; i < BPT; ++i) s_bin[tid + NT * i] = 0u;
     __syncthreads();
-    int all = 0;
+    const int above = shift + bits;  // 32 for the first digit: no bits above
+#pragma unroll 2
+    for (int j = 0; j < steps; ++j) {
+      const uint4 k4 = keys(j);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+      uint32_t d[4];
+      bool in[4];
 #pragma unroll
-    for (int x = 0; x < NW; ++x) all += s_cnt[buf][x];
-    buf ^= 1;  // the next count writes the other row: one barrier a count
-    return all;
-  };
-
-  const int present = count(1u);
-  const int n = present < budget ? present : budget;
-  if (h == 0 && layer == 0 && tid == 0) new_lens[b] = n;
-  uint32_t thr = 1u;
-  int reach = present;  // keys >= thr
-  if (present > n && n > 0) {
-    thr = 0u;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t cand = thr | (1u << bit);
-      const int c = count(cand);
-      if (c >= n) {
-        thr = cand;
-        reach = c;
-        if (c == n) break;
+      for (int e = 0; e < 4; ++e) {
+        in[e] = k[e] != 0u && (above >= 32 || (k[e] >> (above & 31)) == top);
+        d[e] = (k[e] >> shift) & mask;
+      }
+      // one add for a wave whose 256 keys fall in one bin (equal sums, where every
+      // lane's add would wait for the others')
+      const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
+      const bool same = in[0] && in[1] && in[2] && in[3] && d[0] == d0 && d[1] == d0 &&
+                        d[2] == d0 && d[3] == d0;
+      if (__builtin_amdgcn_ballot_w64(!same) == 0) {
+        if (lane == 0) atomicAdd(&s_bin[d0], 256u);
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (in[e]) atomicAdd(&s_bin[d[e]], 1u);
+    }
+    __syncthreads();
+    // thread t has bins kBins - 1 - BPT t downwards: prefix sums from the top
+    uint32_t c[BPT], mine = 0;
+#pragma unroll
+    for (int i = 0; i < BPT; ++i) {
+      c[i] = s_bin[kBins - 1 - (BPT * tid + i)];
+      mine += c[i];
+    }
+    const uint32_t run = wave_prefix(mine);  // inclusive over the wave
+    if (lane == 63) s_sum[w] = run;
+    __syncthreads();
+    uint32_t before = run - mine, total = 0;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const uint32_t v = s_sum[x];
+      if (x < w) before += v;
+      total += v;
+    }
+    if (want > 0 && before < want && want <= before + mine) {  // one thread
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) {
+        if (before < want && want <= before + c[i]) {
+          s_found[0] = (uint32_t)(kBins - 1 - (BPT * tid + i));
+          s_found[1] = c[i];
+          s_found[2] = before;
+          break;
+        }
+        before += c[i];
       }
     }
-  }
-  // wanted among the keys that equal thr (all of them where reach == n)
-  int above = n;
-  if (reach > n) above = thr == 0xffffffffu ? 0 : count(thr + 1u);
-  const int equal = reach > n ? n - above : 0x7fffffff;
+    __syncthreads();
+    return total;
+  };
 
+  // thr and equal: a key is kept above thr, and `equal` of those that equal it
+  uint32_t thr = 0u;
+  int equal = 0;
+  const uint32_t present = digit(21, 11, 0u, (uint32_t)budget);
+  const int n = present < (uint32_t)budget ? (int)present : budget;
+  if (present > (uint32_t)n) {
+    uint32_t top = s_found[0], want = (uint32_t)n - s_found[2];
+    int shift = 21;
+    bool whole = s_found[1] == want;
+    if (!whole) {
+      digit(10, 11, top, want);
+      top = top << 11 | s_found[0], want -= s_found[2], shift = 10;
+      whole = s_found[1] == want;
+      if (!whole) {
+        digit(0, 10, top, want);
+        top = top << 10 | s_found[0], want -= s_found[2], shift = 0;
+      }
+    }
+    // a whole bin: everything from its first key on
+    if (whole) thr = top ? (top << shift) - 1u : 0u;
+    else thr = top, equal = (int)want;
+  }
+  if (h == 0 && layer == 0 && tid == 0) new_lens[b] = n;
+
+  // Places, with the keys that equal the threshold (EQ) or, as usual, without: this
+  // wave's totals, everybody's before it, then its positions in order.
   int32_t* __restrict__ out =
       keep + (((int64_t)layer * gridDim.y + b) * num_kv_heads + h) * budget;
-  __shared__ uint2 s_scan[2][NW];
-  int a0 = 0, e0 = 0;  // above / equal before this chunk
-  int par = 0;
-  if (n > 0) {
-    for_keys([&](int j, const uint32_t (&k)[4]) {
-      if (j >= nj) return;  // workgroup-uniform
-      uint32_t na = 0, ne = 0;
+  auto place = [&](auto with) __attribute__((always_inline)) {
+    constexpr bool EQ = decltype(with)::value;
+    int na = 0, ne = 0;
+#pragma unroll 4
+    for (int j = 0; j < steps; ++j) {
+      const uint4 k4 = keys(j);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        na += k[e] > thr ? 1u : 0u;
-        ne += k[e] == thr ? 1u : 0u;
+        na += __popcll(__builtin_amdgcn_ballot_w64(k[e] > thr));
+        if constexpr (EQ) ne += __popcll(__builtin_amdgcn_ballot_w64(k[e] == thr));
       }
-      uint32_t pa = na, pe = ne;  // inclusive over the wave
+    }
+    if (lane == 0) s_tot[w] = make_int2(na, ne);
+    __syncthreads();
+    int xa = 0, xe = 0;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t ua = __shfl_up(pa, o), ue = __shfl_up(pe, o);
-        if (lane >= o) pa += ua, pe += ue;
-      }
-      if (lane == 63) s_scan[par][w] = make_uint2(pa, pe);
-      __syncthreads();
-      uint32_t ba = 0, be = 0, ta = 0, te = 0;
-#pragma unroll
-      for (int x = 0; x < NW; ++x) {
-        const uint2 v = s_scan[par][x];
-        if (x < w) ba += v.x, be += v.y;
-        ta += v.x, te += v.y;
-      }
-      par ^= 1;
-      int xa = a0 + (int)(ba + pa - na), xe = e0 + (int)(be + pe - ne);
+    for (int x = 0; x < NW; ++x) {
+      const int2 v = s_tot[x];
+      if (x < w) xa += v.x, xe += v.y;
+    }
+#pragma unroll 2
+    for (int j = 0; j < steps; ++j) {
+      const uint4 k4 = keys(j);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+      int la = xa, le = xe;  // before this lane's four
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool up = k[e] > thr, eq = k[e] == thr;
-        if (up || (eq && xe < equal)) out[xa + (xe < equal ? xe : equal)] = 4 * (tid + NT * j) + e;
-        xa += up ? 1 : 0;
-        xe += eq ? 1 : 0;
+        const uint64_t ba = __builtin_amdgcn_ballot_w64(k[e] > thr);
+        la = __builtin_amdgcn_mbcnt_hi((uint32_t)(ba >> 32),
+                                       __builtin_amdgcn_mbcnt_lo((uint32_t)ba, la));
+        xa += __popcll(ba);
+        if constexpr (EQ) {
+          const uint64_t be = __builtin_amdgcn_ballot_w64(k[e] == thr);
+          le = __builtin_amdgcn_mbcnt_hi((uint32_t)(be >> 32),
+                                         __builtin_amdgcn_mbcnt_lo((uint32_t)be, le));
+          xe += __popcll(be);
+        }
       }
-      a0 += (int)ta;
-      e0 += (int)te;
-    });
-  }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool up = k[e] > thr, eq = EQ && k[e] == thr;
+        if (up || (eq && le < equal)) {
+          const int at = EQ ? la + (le < equal ? le : equal) : la;
+          out[at] = 4 * (g0 + 64 * j) + e;
+        }
+        la += up ? 1 : 0;
+        if constexpr (EQ) le += eq ? 1 : 0;
+      }
+    }
+  };
+  if (equal > 0) place(std::true_type{});  // workgroup-uniform
+  else place(std::false_type{});
   for (int i = n + tid; i < budget; i += NT) out[i] = -1;
 }
 
@@ -341,15 +435,14 @@ extern "C" int rkv_evict_select(int32_t* keep, int32_t* new_lens, const float* w
   const int cap = max_context < table ? max_context : table;
   const dim3 grid((unsigned)num_kv_heads, (unsigned)num_seqs, (unsigned)n_layers);
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define RKV_SELECT(NT, J)                                                                        \
-  evict_select_kernel<NT, J><<<grid, NT, 0, s>>>(keep, new_lens, weights, weights_layer_stride,  \
-                                                 block_tables, max_blocks_per_seq, ctx_lens,     \
-                                                 num_kv_heads, num_blocks, budget, sinks, recent, cap)
-  if (cap <= 1024) RKV_SELECT(256, 1);
-  else if (cap <= 4096) RKV_SELECT(1024, 1);
-  else if (cap <= 16384) RKV_SELECT(1024, 4);
-  else if (cap <= 65536) RKV_SELECT(1024, 16);
-  else RKV_SELECT(1024, 0);
+#define RKV_SELECT(NT, K)                                                                      \
+  evict_select_kernel<NT, K><<<grid, NT, K ? (size_t)(cap + 3) / 4 * 16 : 0, s>>>(             \
+      keep, new_lens, weights, weights_layer_stride, block_tables, max_blocks_per_seq, ctx_lens, \
+      num_kv_heads, num_blocks, budget, sinks, recent, cap)
+  // 256 threads up to 4,096 positions, so that several workgroups share a CU
+  if (cap <= 4096) RKV_SELECT(256, true);
+  else if (cap <= kKeysMax) RKV_SELECT(1024, true);
+  else RKV_SELECT(1024, false);
 #undef RKV_SELECT
   return check_launch("rkv_evict_select");
 }

@@ -229,64 +229,149 @@ __global__ __launch_bounds__(256) void decode_merge_rows_kernel(
 }
 
 // ---- accumulated weights -------------------------------------------------------
-// Pass 3 of rkv_decode_attention_weights: the partition pass left every score
-// (log2 domain) and every partition's (m, l); a row's weight is
+// Pass 2 of rkv_decode_attention_weights: the partition pass left every score
+// (log2 domain) and every partition's (m, l, acc); a row's weight is
 //   sum over the group's heads of 2^(score - M_h) / l_h,
-//   M_h = max m_p,  l_h = sum 2^(m_p - M_h) l_p.
-// grid = (chunks of kWeightTokens positions, KV heads, sequences): every
-// workgroup settles its G heads' (M, 1 / l) from the partitions, then a thread
-// takes whole positions (G scores, one 4 G-byte load) and adds their weight to
-// the row's sum.  The adds are hardware atomics: a block of several sequences
-// (a shared prefix) loses none, any other row has a single adder.
+//   M_h = max m_p,  l_h = sum 2^(m_p - M_h) l_p,
+// and a head's output the merge's.  grid = (MG + chunks of kWeightTokens positions,
+// KV heads, sequences): the first MG workgroups of a (KV head, sequence) merge its
+// heads -- one workgroup with a wave a head where there are few partitions, else a
+// workgroup a head -- and the others add up weights: a thread requests its
+// positions' scores (4 G bytes each) and block ids, all heads' (M, 1 / l) are settled
+// from the partitions meanwhile, and the weight is added to the row's sum.  The
+// adds are hardware atomics: a block of several sequences (a shared prefix) loses
+// none, any other row has a single adder.
+// At 64 x U[512, 4096] the scores are 20 MB beside 635 MB of K and V.  Writing them
+// costs the partition pass 19 us (104 to 123): all workgroups writing one place
+// cost nothing, a quarter of the bytes 6 us, half 13, so it is where the rows land
+// in memory, not the stores; streaming and write-through hints made it no faster.
 constexpr int kWeightTokens = 1024;
+constexpr int kWaveMergeParts = 16;  // up to so many partitions a wave merges a head
 
-template <int G>
-__global__ __launch_bounds__(256) void decode_weights_kernel(
-    float* __restrict__ weights, const float* __restrict__ scores,
-    const float* __restrict__ part_ml, const int32_t* __restrict__ block_tables,
-    int max_blocks_per_seq, const int32_t* __restrict__ ctx_lens, int ctx_cap, int num_kv_heads,
-    int64_t num_blocks, int P, int max_parts) {
+template <int G, int D>
+__global__ __launch_bounds__(256) void decode_merge_weights_kernel(
+    float* __restrict__ out, float* __restrict__ weights, const float* __restrict__ scores,
+    const float* __restrict__ part_acc, const float* __restrict__ part_ml,
+    const int32_t* __restrict__ block_tables, int max_blocks_per_seq,
+    const int32_t* __restrict__ ctx_lens, int ctx_cap, int num_kv_heads, int64_t num_blocks, int P,
+    int max_parts) {
+  constexpr int V4 = D / 4, RPW = 64 / V4;  // float4 a partition row, rows a wave
+  constexpr int NU = kWeightTokens / 256;   // positions a thread
   __shared__ float s_m[G], s_inv[G];
+  __shared__ __align__(16) float s_acc[4][D];
   const int kh = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const bool few = max_parts <= kWaveMergeParts;
+  const int mg = few ? 1 : G;  // workgroups that merge
   int L = ctx_lens[b];
   L = L < 0 ? 0 : (L > ctx_cap ? ctx_cap : L);
-  const int t0 = blockIdx.x * kWeightTokens;
-  if (t0 >= L) return;
+  const int64_t head0 = ((int64_t)b * num_kv_heads + kh) * G;
+  const int64_t row0 = head0 * max_parts;  // partition 0 of head 0
   const int np = (L + P - 1) / P;
-  for (int g = w; g < G; g += 4) {  // a wave a head
-    const float* ml =
-        part_ml + (((int64_t)b * num_kv_heads + kh) * G + g) * max_parts * 2;
-    float M = -INFINITY;
+
+  // a head's (M, 1 / l), in every lane
+  auto settle = [&](int g, float& M, float& inv) __attribute__((always_inline)) {
+    const float* ml = part_ml + (row0 + (int64_t)g * max_parts) * 2;
+    M = -INFINITY;
     for (int p = lane; p < np; p += 64) M = fmaxf(M, ml[2 * p]);
     M = wave_max(M);
     float l = 0.0f;
     for (int p = lane; p < np; p += 64)
       l += ml[2 * p] == -INFINITY ? 0.0f : exp2f(ml[2 * p] - M) * ml[2 * p + 1];
     l = wave_sum(l);
-    if (lane == 0) {
-      s_m[g] = M;
-      s_inv[g] = l > 0.0f ? 1.0f / l : 0.0f;
+    inv = l > 0.0f ? 1.0f / l : 0.0f;
+  };
+  // partitions p0, p0 + step, .. of a head, weighted; the sum over the wave's rows
+  // in the lanes of row 0
+  auto merge = [&](int g, float M, int p0, int step) __attribute__((always_inline)) {
+    const int64_t row = row0 + (int64_t)g * max_parts;
+    const int c = lane % V4;
+    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int p = p0 + lane / V4; p < np; p += step) {
+      const float m = part_ml[(row + p) * 2];
+      const float wgt = m == -INFINITY ? 0.0f : exp2f(m - M);
+      const float4 a = *reinterpret_cast<const float4*>(part_acc + (row + p) * D + 4 * c);
+      num.x = fmaf(wgt, a.x, num.x);
+      num.y = fmaf(wgt, a.y, num.y);
+      num.z = fmaf(wgt, a.z, num.z);
+      num.w = fmaf(wgt, a.w, num.w);
     }
+#pragma unroll
+    for (int o = V4; o < 64; o <<= 1) {
+      num.x += __shfl_xor(num.x, o);
+      num.y += __shfl_xor(num.y, o);
+      num.z += __shfl_xor(num.z, o);
+      num.w += __shfl_xor(num.w, o);
+    }
+    return num;
+  };
+
+  if ((int)blockIdx.x < mg) {
+    if (np <= 1) return;  // finished by the partition pass
+    if (few) {
+      for (int g = w; g < G; g += 4) {
+        float M, inv;
+        settle(g, M, inv);
+        const float4 num = merge(g, M, 0, RPW);
+        if (lane < V4)
+          *reinterpret_cast<float4*>(out + (head0 + g) * D + 4 * lane) =
+              make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv);
+      }
+      return;
+    }
+    const int g = blockIdx.x;
+    float M, inv;
+    settle(g, M, inv);
+    const float4 num = merge(g, M, w * RPW, 4 * RPW);
+    if (lane < V4) *reinterpret_cast<float4*>(&s_acc[w][4 * lane]) = num;
+    __syncthreads();
+    if (tid < D)
+      out[(head0 + g) * D + tid] =
+          ((s_acc[0][tid] + s_acc[1][tid]) + (s_acc[2][tid] + s_acc[3][tid])) * inv;
+    return;
+  }
+
+  const int t0 = ((int)blockIdx.x - mg) * kWeightTokens;
+  if (t0 >= L) return;
+  const float* sp = scores + head0 * ((int64_t)max_parts * P);
+  const int32_t* tab = block_tables + (int64_t)b * max_blocks_per_seq;
+  float s[NU][G];
+  int32_t blk[NU];
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    const int t = t0 + tid + 256 * u;
+    const int64_t tc = t < L ? t : L - 1;  // past the end: the last position, not added
+    if constexpr (G % 4 == 0) {
+#pragma unroll
+      for (int g = 0; g < G; g += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(sp + tc * G + g);
+        s[u][g] = v.x, s[u][g + 1] = v.y, s[u][g + 2] = v.z, s[u][g + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < G; ++g) s[u][g] = sp[tc * G + g];
+    }
+    blk[u] = t < L ? tab[tc / kBS] : -1;
+  }
+  for (int g = w; g < G; g += 4) {  // a wave a head
+    float M, inv;
+    settle(g, M, inv);
+    if (lane == 0) s_m[g] = M, s_inv[g] = inv;
   }
   __syncthreads();
   float M[G], inv[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) M[g] = s_m[g], inv[g] = s_inv[g];
-  const float* sp =
-      scores + (((int64_t)b * num_kv_heads + kh) * ((int64_t)max_parts * P)) * G;
-  const int32_t* tab = block_tables + (int64_t)b * max_blocks_per_seq;
-  const int t1 = L < t0 + kWeightTokens ? L : t0 + kWeightTokens;
-  for (int t = t0 + tid; t < t1; t += 256) {
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
     float sum = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float s = sp[(int64_t)t * G + g];
-      sum += s == -INFINITY ? 0.0f : exp2f(s - M[g]) * inv[g];
-    }
-    const int32_t blk = tab[t / kBS];
-    if (blk >= 0 && blk < num_blocks)
-      unsafeAtomicAdd(weights + ((int64_t)blk * num_kv_heads + kh) * kBS + t % kBS, sum);
+    for (int g = 0; g < G; ++g)
+      sum += s[u][g] == -INFINITY ? 0.0f : exp2f(s[u][g] - M[g]) * inv[g];
+    if (blk[u] >= 0 && blk[u] < num_blocks)
+      unsafeAtomicAdd(weights + ((int64_t)blk[u] * num_kv_heads + kh) * kBS +
+                          (t0 + tid + 256 * u) % kBS, sum);
   }
 }
 
@@ -890,14 +975,12 @@ WeightsWs weights_ws(int B, int Hq, int D, int64_t max_parts, int64_t tokens) {
   return w;
 }
 
-// Partition sizes with a score build (decode_stream.hpp): the shape's pick, at
-// most the largest 4-wave build's.
+// Partition sizes with a score build (decode_stream.hpp).
 int weights_part(int dtype, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
                  int cap) {
   if (cap <= kShortP) return kShortP;
   if (cap <= kSmallP) return kSmallP;
-  const int P = shape_part(dtype, num_seqs, num_q_heads, num_kv_heads, head_dim, cap);
-  return P < kP ? P : kP;
+  return shape_part(dtype, num_seqs, num_q_heads, num_kv_heads, head_dim, cap);
 }
 
 }  // namespace
@@ -915,7 +998,7 @@ extern "C" size_t rkv_decode_weights_workspace_bytes(int num_seqs, int num_q_hea
   if (max_context > kSmallP && kTinyGroups / groups > 0)
     tiny = std::min({parts(kShortP), (int64_t)kTinyParts, (int64_t)kTinyGroups / groups});
   return weights_ws(num_seqs, num_q_heads, head_dim, std::max(parts(kSmallP), tiny),
-                    (int64_t)max_context + kP)
+                    (int64_t)max_context + kWideP2)
       .total;
 }
 
@@ -957,22 +1040,27 @@ extern "C" int rkv_decode_attention_weights(
                      num_kv_heads, num_blocks, scale * kLog2e, max_parts, P2 / (kBS * l.nw),
                      nullptr, nullptr, scores);
   if (int rc = check_launch("decode_stream_kernel")) return rc;
-  if (int rc = launch_merge(out, ctx_lens, num_seqs, num_q_heads, head_dim, cap, P2, max_parts,
-                            workspace, a.stream))
-    return rc;
   if (cap <= 0) return RKV_OK;
-  const dim3 wgrid((unsigned)((cap + kWeightTokens - 1) / kWeightTokens), (unsigned)num_kv_heads,
-                   (unsigned)num_seqs);
-#define RKV_WEIGHTS(GG)                                                                         \
-  decode_weights_kernel<GG><<<wgrid, 256, 0, a.stream>>>(weights, scores, ml, block_tables,     \
-                                                         max_blocks_per_seq, ctx_lens, cap,     \
-                                                         num_kv_heads, num_blocks, P2, max_parts)
+  const int mg = max_parts <= kWaveMergeParts ? 1 : G;
+  const dim3 wgrid((unsigned)(mg + (cap + kWeightTokens - 1) / kWeightTokens),
+                   (unsigned)num_kv_heads, (unsigned)num_seqs);
+#define RKV_WEIGHTS(GG, DD)                                                                     \
+  decode_merge_weights_kernel<GG, DD><<<wgrid, 256, 0, a.stream>>>(                             \
+      out, weights, scores, acc, ml, block_tables, max_blocks_per_seq, ctx_lens, cap,           \
+      num_kv_heads, num_blocks, P2, max_parts)
+#define RKV_WEIGHTS_D(GG)                        \
+  do {                                           \
+    if (head_dim == 32) RKV_WEIGHTS(GG, 32);     \
+    else if (head_dim == 64) RKV_WEIGHTS(GG, 64); \
+    else RKV_WEIGHTS(GG, 128);                   \
+  } while (0)
   switch (G) {
-    case 1: RKV_WEIGHTS(1); break;
-    case 2: RKV_WEIGHTS(2); break;
-    case 4: RKV_WEIGHTS(4); break;
-    default: RKV_WEIGHTS(8); break;
+    case 1: RKV_WEIGHTS_D(1); break;
+    case 2: RKV_WEIGHTS_D(2); break;
+    case 4: RKV_WEIGHTS_D(4); break;
+    default: RKV_WEIGHTS_D(8); break;
   }
+#undef RKV_WEIGHTS_D
 #undef RKV_WEIGHTS
-  return check_launch("decode_weights_kernel");
+  return check_launch("decode_merge_weights_kernel");
 }

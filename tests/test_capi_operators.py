@@ -128,17 +128,17 @@ def test_decode_attention_weights_workspace_holds_every_shape():
     L = _lib.lib()
     for B, hkv, g in [(1, 1, 1), (1, 8, 4), (2, 8, 4), (3, 2, 8), (16, 1, 4), (64, 8, 4), (300, 1, 1)]:
         for maxc in (1, 16, 128, 129, 512, 513, 640, 1000, 4096, 16384, 32768, 65536, 131072):
-            need = L.rkv_decode_weights_workspace_bytes(B, g * hkv, hkv, 64, maxc)
+            need = L.rkv_decode_weights_workspace_bytes(B, g * hkv, hkv, 128, maxc)
             assert need > 0
             for cap in {maxc, max(1, maxc - 1), max(1, maxc // 2), min(maxc, 520)}:
                 # a null query is reported after the workspace of the partials, the
                 # scores' share is checked by arithmetic
-                p = L.rkv_decode_partition_size_for(0, B, g * hkv, hkv, 64, RKV_BF16, cap)
-                p = 128 if cap <= 128 else 512 if cap <= 512 else min(p, 640)
+                p = L.rkv_decode_partition_size_for(0, B, g * hkv, hkv, 128, RKV_BF16, cap)
+                p = 128 if cap <= 128 else 512 if cap <= 512 else p
                 parts = -(-cap // p)
                 rows = B * g * hkv
                 pad = lambda x: -(-x // 256) * 256  # noqa: E731
-                used = pad(rows * parts * 64 * 4) + pad(rows * parts * 8) + rows * parts * p * 4
+                used = pad(rows * parts * 128 * 4) + pad(rows * parts * 8) + rows * parts * p * 4
                 assert used <= need, (B, hkv, g, maxc, cap)
 
 

@@ -129,9 +129,10 @@ def test_append_block_q_borders(dev, fmt):
     v, ks, vs = k.copy(), np.ones((nb, hkv), f), np.ones((nb, hkv), f)
     tables = np.arange(seqs, dtype=np.int32)[:, None]
     start = (4 * np.arange(seqs + 1)).astype(np.int32)
-    for at in (0, 6):                       # fresh, then behind six rows
+    for at, by in ((0, 1.0), (6, 1.0), (10, 24.0)):   # fresh, behind six rows, a growth
         ctx = np.full(seqs, at + 4, np.int32)
-        new = rows.reshape(-1, hkv, d)
+        with np.errstate(over="ignore"):
+            new = (rows * f(by)).reshape(-1, hkv, d)
         g = [to_dev(a, dev) for a in (k, v, ks, vs)]
         kv.append_block_q(*g, to_dev(new, dev), to_dev(new[::-1].copy(), dev), to_dev(start, dev),
                           to_dev(tables, dev), to_dev(ctx, dev), fmt, max_new=4)
