@@ -7,6 +7,7 @@ block_size, D]`` for multi-layer append/copy) in float32 or bfloat16.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -44,6 +45,13 @@ def _dev(t: torch.Tensor, name: str, dtype=None) -> torch.Tensor:
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t
+
+
+def _one_device(dev: int, named) -> None:
+    """Every tensor on device `dev`: a kernel is launched on one device's stream."""
+    for t, name in named:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} must be on the call's device")
 
 
 def check_attention_shapes(q_shape, pool_shape, tables_shape, lens_shape,
@@ -155,6 +163,9 @@ def copy_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, pairs: torch.Tensor)
                                 _stream(k_pool)))
 
 
+# A size is a function of the shape alone: asking the library again costs 0.8 of a
+# small call's 8 us on the host.
+@functools.lru_cache(maxsize=4096)
 def workspace_bytes(num_seqs: int, num_q_heads: int, head_dim: int, max_context: int,
                     partition_size: int = 0) -> int:
     return int(lib().rkv_decode_workspace_bytes(num_seqs, num_q_heads, head_dim, max_context,
@@ -303,14 +314,18 @@ def _bcode(fmt) -> int:
     return _BFMT[fmt]
 
 
-def _scale_pools(k_pool, v_pool, k_scale, v_scale, code: int) -> None:
+def _scale_shapes(k_shape, v_shape, ks_shape, vs_shape, code: int) -> None:
     """Scale pools of the shape their format has: one a row, or one a tile.  The
     kernels index them by the byte pools' shape."""
-    _dev(k_scale, "k_scale", torch.float32), _dev(v_scale, "v_scale", torch.float32)
     cut = -2 if code >= _lib.RKV_I8_BLOCK else -1
-    if k_scale.shape != k_pool.shape[:cut] or v_scale.shape != v_pool.shape[:cut]:
+    if ks_shape != k_shape[:cut] or vs_shape != v_shape[:cut]:
         raise ValueError("scale pools must be the byte pools' shape without head_dim, and for the "
                          "block formats without the rows too")
+
+
+def _scale_pools(k_pool, v_pool, k_scale, v_scale, code: int) -> None:
+    _dev(k_scale, "k_scale", torch.float32), _dev(v_scale, "v_scale", torch.float32)
+    _scale_shapes(k_pool.shape, v_pool.shape, k_scale.shape, v_scale.shape, code)
 
 
 def _workspace_bytes_q(num_seqs: int, num_q_heads: int, head_dim: int, max_context: int,
@@ -443,16 +458,29 @@ def decode_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     the size to ask for if a small call wants finer partitions; its pick over
     block-scaled ones."""
     code = _anycode(fmt)
-    _dev(q, "q", torch.float32), _dev(k_pool, "k_pool", torch.uint8)
-    _dev(v_pool, "v_pool", torch.uint8), _dev(k_scale, "k_scale", torch.float32)
-    _dev(v_scale, "v_scale", torch.float32)
-    _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
-    nb, hkv, bs, d = k_pool.shape
+    u8, f32, i32 = torch.uint8, torch.float32, torch.int32
+    dev = q.get_device()
+    if not (q.dtype is f32 and k_pool.dtype is u8 and v_pool.dtype is u8 and
+            k_scale.dtype is f32 and v_scale.dtype is f32 and block_tables.dtype is i32 and
+            ctx_lens.dtype is i32 and q.is_contiguous() and k_pool.is_contiguous() and
+            v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous() and
+            block_tables.is_contiguous() and ctx_lens.is_contiguous() and dev >= 0 and
+            dev == k_pool.get_device() == v_pool.get_device() == k_scale.get_device() ==
+            v_scale.get_device() == block_tables.get_device() == ctx_lens.get_device()):
+        _dev(q, "q", f32), _dev(k_pool, "k_pool", u8)  # says which and why
+        _dev(v_pool, "v_pool", u8), _dev(k_scale, "k_scale", f32)
+        _dev(v_scale, "v_scale", f32)
+        _dev(block_tables, "block_tables", i32), _dev(ctx_lens, "ctx_lens", i32)
+        _one_device(dev, ((k_pool, "k_pool"), (v_pool, "v_pool"), (k_scale, "k_scale"),
+                          (v_scale, "v_scale"), (block_tables, "block_tables"),
+                          (ctx_lens, "ctx_lens")))
+    shape, tables = k_pool.shape, block_tables.shape
+    nb, hkv, bs, d = shape
     if code >= _lib.RKV_I8_BLOCK:
-        _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
-    check_attention_shapes(q.shape, k_pool.shape, block_tables.shape, ctx_lens.shape)
+        _scale_shapes(shape, v_pool.shape, k_scale.shape, v_scale.shape, code)
+    check_attention_shapes(q.shape, shape, tables, ctx_lens.shape)
     B, hq, _ = q.shape
-    mbs = block_tables.shape[1]
+    mbs = tables[1]
     if max_context is None:
         max_context = mbs * bs
     if scale is None:
@@ -469,7 +497,7 @@ def decode_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
                                        v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                        block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, hq,
                                        hkv, d, bs, nb, max_context, float(scale), code,
-                                       partition_size, ws_ptr, ws_len, _stream(q)))
+                                       partition_size, ws_ptr, ws_len, _raw_stream(dev)))
     return out
 
 
@@ -520,32 +548,49 @@ def append_block_q(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Te
     (computed from new_start, with a device sync, when not given).
     """
     code = _bcode(fmt)
-    _dev(k_pool, "k_pool", torch.uint8), _dev(v_pool, "v_pool", torch.uint8)
-    _dev(k_new, "k_new", torch.float32), _dev(v_new, "v_new", torch.float32)
-    _dev(new_start, "new_start", torch.int32), _dev(block_tables, "block_tables", torch.int32)
-    _dev(ctx_lens, "ctx_lens", torch.int32)
-    _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
-    multi = k_pool.dim() == 5
-    n_layers = k_pool.shape[0] if multi else 1
-    nb, hkv, bs, d = k_pool.shape[-4:]
-    if k_new.shape != v_new.shape or k_pool.shape != v_pool.shape:
+    u8, f32, i32 = torch.uint8, torch.float32, torch.int32
+    dev = k_pool.get_device()
+    if not (k_pool.dtype is u8 and v_pool.dtype is u8 and k_scale.dtype is f32 and
+            v_scale.dtype is f32 and k_new.dtype is f32 and v_new.dtype is f32 and
+            new_start.dtype is i32 and block_tables.dtype is i32 and ctx_lens.dtype is i32 and
+            k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and
+            v_scale.is_contiguous() and k_new.is_contiguous() and v_new.is_contiguous() and
+            new_start.is_contiguous() and block_tables.is_contiguous() and
+            ctx_lens.is_contiguous() and dev >= 0 and
+            dev == v_pool.get_device() == k_scale.get_device() == v_scale.get_device() ==
+            k_new.get_device() == v_new.get_device() == new_start.get_device() ==
+            block_tables.get_device() == ctx_lens.get_device()):
+        _dev(k_pool, "k_pool", u8), _dev(v_pool, "v_pool", u8)  # says which and why
+        _dev(k_scale, "k_scale", f32), _dev(v_scale, "v_scale", f32)
+        _dev(k_new, "k_new", f32), _dev(v_new, "v_new", f32)
+        _dev(new_start, "new_start", i32), _dev(block_tables, "block_tables", i32)
+        _dev(ctx_lens, "ctx_lens", i32)
+        _one_device(dev, ((v_pool, "v_pool"), (k_scale, "k_scale"), (v_scale, "v_scale"),
+                          (k_new, "k_new"), (v_new, "v_new"), (new_start, "new_start"),
+                          (block_tables, "block_tables"), (ctx_lens, "ctx_lens")))
+    shape = k_pool.shape
+    multi = len(shape) == 5
+    n_layers = shape[0] if multi else 1
+    nb, hkv, bs, d = shape[-4:]
+    if shape != v_pool.shape or k_new.shape != v_new.shape:
         raise ValueError("K and V shapes differ")
-    if k_new.shape[-2:] != (hkv, d) or k_new.dim() != (4 if multi else 3) or \
-            (multi and k_new.shape[0] != n_layers):
-        raise ValueError(f"k_new shape {tuple(k_new.shape)} does not match pool {tuple(k_pool.shape)}")
-    B = ctx_lens.shape[0]
-    if ctx_lens.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != B or \
-            new_start.shape != (B + 1,):
+    if k_scale.shape != shape[:-2] or v_scale.shape != shape[:-2]:
+        raise ValueError("scale pools must be the byte pools' shape without rows and head_dim")
+    *lead, total, rh, rd = k_new.shape
+    if rh != hkv or rd != d or lead != ([n_layers] if multi else []):
+        raise ValueError(f"k_new shape {tuple(k_new.shape)} does not match pool {tuple(shape)}")
+    (B,) = ctx_lens.shape
+    rows, mbs = block_tables.shape
+    if rows != B or new_start.shape != (B + 1,):
         raise ValueError("one block-table row and one length per sequence, new_start B + 1 offsets")
     if max_new is None:
         max_new = int((new_start[1:] - new_start[:-1]).max().item()) if B else 0
-    total = k_new.shape[-3]
     check(lib().rkv_append_block_q(
         k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
         nb * hkv * bs * d if multi else 0, k_new.data_ptr(), v_new.data_ptr(),
         total * hkv * d if multi else 0, hkv * d, d, new_start.data_ptr(),
-        block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, n_layers, hkv, d,
-        bs, nb, max_new, code, _stream(k_pool)))
+        block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, n_layers, hkv, d, bs, nb, max_new,
+        code, _raw_stream(dev)))
 
 
 def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -561,6 +606,9 @@ def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
     _dev(v_pool, "v_pool", torch.uint8), _dev(q_start, "q_start", torch.int32)
     _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
     _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
+    _one_device(q.get_device(), ((k_pool, "k_pool"), (v_pool, "v_pool"), (k_scale, "k_scale"),
+                                 (v_scale, "v_scale"), (q_start, "q_start"),
+                                 (block_tables, "block_tables"), (ctx_lens, "ctx_lens")))
     check_attention_shapes(q.shape, k_pool.shape, block_tables.shape, ctx_lens.shape,
                            q_start.shape)
     nb, hkv, bs, d = k_pool.shape
@@ -613,8 +661,13 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def _rope_shapes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> None:
+def _rope_tensors(positions: torch.Tensor, inv_freq: torch.Tensor) -> None:
     _dev(positions, "positions", torch.int32), _dev(inv_freq, "inv_freq", torch.float64)
+
+
+def _rope_shapes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor) -> None:
+    _rope_tensors(positions, inv_freq)
+    _one_device(x.get_device(), ((positions, "positions"), (inv_freq, "inv_freq")))
     if positions.shape != (x.shape[0],):
         raise ValueError(f"{tuple(positions.shape)} positions for {x.shape[0]} tokens")
     if inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > x.shape[2]:
@@ -632,8 +685,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
     _rope_shapes(x, positions, inv_freq)
     if out is None:
         out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-    elif _rows(out, "out").shape != x.shape:
-        raise ValueError("out must have x's shape")
+    elif _rows(out, "out").shape != x.shape or out.get_device() != x.get_device():
+        raise ValueError("out must have x's shape, on its device")
     t, h, d = x.shape
     check(lib().rkv_rope(out.data_ptr(), x.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
                          t, h, d, 2 * inv_freq.shape[0], out.stride(0), out.stride(1),
@@ -650,21 +703,39 @@ def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     pools get what append (fp32 and bf16 pools) or append_q (fmt 'int8' or 'fp8',
     with the scale pools) of rope(k_new) and v_new writes.  Shapes as append's and
     rope's; out may be q."""
-    _rows(q, "q"), _rows(k_new, "k_new"), _rows(v_new, "v_new")
-    _rope_shapes(q, positions, inv_freq)
-    _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool")
-    _dev(slot_mapping, "slot_mapping", torch.int64)
-    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+    f32 = torch.float32
+    dev = q.get_device()
+    qs, ns, vs_ = q.stride(), k_new.stride(), v_new.stride()
+    if not (q.dtype is f32 and k_new.dtype is f32 and v_new.dtype is f32 and
+            positions.dtype is torch.int32 and inv_freq.dtype is torch.float64 and
+            slot_mapping.dtype is torch.int64 and qs[-1] == 1 and ns[-1] == 1 and
+            vs_[-1] == 1 and positions.is_contiguous() and inv_freq.is_contiguous() and
+            slot_mapping.is_contiguous() and k_pool.is_contiguous() and
+            v_pool.is_contiguous() and dev >= 0 and
+            dev == k_new.get_device() == v_new.get_device() == positions.get_device() ==
+            inv_freq.get_device() == k_pool.get_device() == v_pool.get_device() ==
+            slot_mapping.get_device()):
+        _rows(q, "q"), _rows(k_new, "k_new"), _rows(v_new, "v_new")  # says which and why
+        _rope_tensors(positions, inv_freq)
+        _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool")
+        _dev(slot_mapping, "slot_mapping", torch.int64)
+        _one_device(dev, ((k_new, "k_new"), (v_new, "v_new"), (positions, "positions"),
+                          (inv_freq, "inv_freq"), (k_pool, "k_pool"), (v_pool, "v_pool"),
+                          (slot_mapping, "slot_mapping")))
+    shape, qshape, nshape = k_pool.shape, q.shape, k_new.shape
+    if len(shape) != 4 or shape != v_pool.shape or k_pool.dtype is not v_pool.dtype:
         raise ValueError("k_pool and v_pool must be one layer's pools of one shape and type")
-    nb, hkv, bs, d = k_pool.shape
-    t, hq, dq = q.shape
-    if k_new.shape != (t, hkv, d) or v_new.shape != (t, hkv, d) or dq != d:
-        raise ValueError(f"q {tuple(q.shape)}, k_new {tuple(k_new.shape)}, v_new "
-                         f"{tuple(v_new.shape)} do not match pool {tuple(k_pool.shape)}")
-    if k_new.stride() != v_new.stride():
+    nb, hkv, bs, d = shape
+    t, hq, dq = qshape
+    if nshape != (t, hkv, d) or v_new.shape != nshape or dq != d:
+        raise ValueError(f"q {tuple(qshape)}, k_new {tuple(nshape)}, v_new "
+                         f"{tuple(v_new.shape)} do not match pool {tuple(shape)}")
+    if ns != vs_:
         raise ValueError("k_new and v_new must have the same strides")
-    if slot_mapping.shape != (t,):
-        raise ValueError("slot_mapping must be [n_tokens]")
+    (half,) = inv_freq.shape
+    if positions.shape != (t,) or slot_mapping.shape != (t,) or 2 * half > d:
+        raise ValueError("positions and slot_mapping must be [n_tokens], inv_freq "
+                         "[rotary_dim / 2] with rotary_dim <= head_dim")
     if fmt is None:
         code, ks, vs = _dtype_code(k_pool), None, None
     else:
@@ -673,22 +744,26 @@ def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
         if k_scale is None or v_scale is None:
             raise ValueError("1-byte pools need their scale pools")
         _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
+        _one_device(dev, ((k_scale, "k_scale"), (v_scale, "v_scale")))
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    elif _rows(out, "out").shape != q.shape:
-        raise ValueError("out must have q's shape")
+        out = torch.empty(qshape, dtype=f32, device=q.device)
+        os = out.stride()
+    else:
+        os = out.stride()
+        if out.shape != qshape or out.dtype is not f32 or os[-1] != 1 or out.get_device() != dev:
+            raise ValueError("out must be fp32 of q's shape with contiguous rows, on its device")
     check(lib().rkv_rope_append(
         out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks, vs, q.data_ptr(),
-        k_new.data_ptr(), v_new.data_ptr(), out.stride(0), out.stride(1), q.stride(0),
-        q.stride(1), k_new.stride(0), k_new.stride(1), positions.data_ptr(), inv_freq.data_ptr(),
-        slot_mapping.data_ptr(), t, hq, hkv, d, 2 * inv_freq.shape[0], int(interleaved),
-        magnitude, bs, nb, code, _stream(q)))
+        k_new.data_ptr(), v_new.data_ptr(), os[0], os[1], qs[0], qs[1], ns[0], ns[1],
+        positions.data_ptr(), inv_freq.data_ptr(), slot_mapping.data_ptr(), t, hq, hkv, d,
+        2 * half, int(interleaved), magnitude, bs, nb, code, _raw_stream(dev)))
     return out
 
 
 # ---- eviction by accumulated attention weight ------------------------------------
 
+@functools.lru_cache(maxsize=4096)
 def weights_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
                             max_context: int) -> int:
     return int(lib().rkv_decode_weights_workspace_bytes(num_seqs, num_q_heads, num_kv_heads,
@@ -726,6 +801,9 @@ def decode_attention_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
     if weights.shape != k_pool.shape[:3]:
         raise ValueError("weights must be the pools' shape without head_dim")
     code, ks, vs = _pool_code(k_pool, v_pool, k_scale, v_scale, fmt)
+    _one_device(q.get_device(), ((k_pool, "k_pool"), (v_pool, "v_pool"), (weights, "weights"),
+                                 (block_tables, "block_tables"), (ctx_lens, "ctx_lens"),
+                                 (k_scale, "k_scale"), (v_scale, "v_scale")))
     nb, hkv, bs, d = k_pool.shape
     B, hq, _ = q.shape
     mbs = block_tables.shape[1]
@@ -759,6 +837,8 @@ def evict_select(weights: torch.Tensor, block_tables: torch.Tensor, ctx_lens: to
     if weights.dim() not in (3, 4) or block_tables.dim() != 2 or ctx_lens.dim() != 1 or \
             block_tables.shape[0] != ctx_lens.shape[0]:
         raise ValueError("weights [.., num_blocks, Hkv, 16], one table row and length a sequence")
+    _one_device(weights.get_device(), ((block_tables, "block_tables"), (ctx_lens, "ctx_lens"),
+                                       (keep, "keep"), (new_lens, "new_lens")))
     n_layers = weights.shape[0] if weights.dim() == 4 else 1
     nb, hkv, bs = weights.shape[-3:]
     B, mbs = block_tables.shape
@@ -793,6 +873,10 @@ def evict_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, keep: torch.Tensor
     if k_pool.dim() not in (4, 5):
         raise ValueError("pools must be [num_blocks, Hkv, 16, D] or [n_layers, ..]")
     code, ks, vs = _pool_code(k_pool, v_pool, k_scale, v_scale, fmt)
+    _one_device(k_pool.get_device(), ((v_pool, "v_pool"), (keep, "keep"), (new_lens, "new_lens"),
+                                      (src_tables, "src_tables"), (dst_tables, "dst_tables"),
+                                      (k_scale, "k_scale"), (v_scale, "v_scale"),
+                                      (weights, "weights")))
     nb, hkv, bs, d = k_pool.shape[-4:]
     n_layers = k_pool.shape[0] if k_pool.dim() == 5 else 1
     B = new_lens.shape[0]

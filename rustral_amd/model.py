@@ -6,13 +6,14 @@ csrc/decoder.hip).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import numpy as np
 import torch
 
 from ._lib import RkvError, check, lib
-from .kv import _dev, _dtype_code, _stream
+from .kv import _dev, _dtype_code, _raw_stream, _stream
 
 
 class DecoderConfig(C.Structure):
@@ -385,53 +386,67 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     the offsets bias_start; allowed holds a bit a token in int32 words
     [rows, >= ceil(vocab / 32)].  The pick is argmax's, -1 where a row has
     nothing left.  out may be logits.  rkv_process_logits has the formulas."""
-    _matrix(logits, "logits")
+    f32, i32 = torch.float32, torch.int32
+    dev = logits.get_device()
+    if not (dev >= 0 and logits.dtype is f32 and logits.dim() == 2):
+        _matrix(logits, "logits")  # says why
     rows, n = logits.shape
-    dev = logits.device
+    stride = logits.stride()
+    if stride[1] != 1 and n > 1:
+        _matrix(logits, "logits")
 
-    def ptr(t, name, dtype, shape):
+    def ptr(t, name, dtype, length):
+        """A vector's address, None without one."""
         if t is None:
             return None
-        if _dev(t, name, dtype).shape != shape:
-            raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+        if not (t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and
+                t.shape == (length,)):
+            _dev(t, name, dtype)
+            raise ValueError(f"{name} must be [{length}] on the logits' device, got {list(t.shape)}")
         return t.data_ptr()
 
-    per, ends = (rows,), (rows + 1,)
-    if allowed is not None and (_dev(allowed, "allowed", torch.int32).dim() != 2 or
-                                allowed.shape[0] != rows or allowed.shape[1] < -(-n // 32)):
-        raise ValueError(f"allowed must be [{rows}, {-(-n // 32)}] words or wider")
-    if bias_ids is not None and (bias is None or bias_start is None or
-                                 bias_ids.shape != bias.shape or bias_ids.dim() != 1):
-        raise ValueError("bias_ids needs bias of the same length and bias_start")
-    if history is not None and _dev(history, "history", torch.int32).dim() != 1:
-        raise ValueError("history must be one row of token ids")
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.float32, device=dev)
-    elif _matrix(out, "out").shape != logits.shape:
-        raise ValueError("out must have the logits' shape")
+        out = torch.empty((rows, n), dtype=f32, device=logits.device)
+    ostride = out.stride()
+    if out.dtype is not f32 or out.shape != (rows, n) or out.get_device() != dev or \
+            (ostride[1] != 1 and n > 1):
+        raise ValueError("out must be fp32 of the logits' shape with contiguous rows, on their device")
     if pick is None:
-        pick = torch.empty(rows, dtype=torch.int32, device=dev)
-    if workspace is None:
-        need = lib().rkv_process_logits_workspace_bytes(rows, n)
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        pick = torch.empty(rows, dtype=i32, device=logits.device)
+    ws_bytes, ws = _logits_workspace(rows, n), None
+    if workspace is not None:
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif ws_bytes:
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
+        ws = workspace.data_ptr()
+    words = 0
+    if allowed is not None:
+        if allowed.dtype is not i32 or not allowed.is_contiguous() or \
+                allowed.get_device() != dev or allowed.dim() != 2 or allowed.shape[0] != rows:
+            _dev(allowed, "allowed", i32)
+            raise ValueError(f"allowed must be [{rows}, words] on the logits' device")
+        words = allowed.shape[1]
+        if words < -(-n // 32):
+            raise ValueError(f"allowed must be [{rows}, {-(-n // 32)}] words or wider")
+    if bias_ids is not None and (bias is None or bias_start is None):
+        raise ValueError("bias_ids needs bias of the same length and bias_start")
+    entries = 0 if bias_ids is None else bias_ids.numel()
     check(lib().rkv_process_logits(
-        out.data_ptr(), out.stride(0), ptr(pick, "pick", torch.int32, per), logits.data_ptr(),
-        logits.stride(0), rows, n, None if history is None else history.data_ptr(),
-        ptr(history_start, "history_start", torch.int32, ends),
-        ptr(prompt_lens, "prompt_lens", torch.int32, per),
-        ptr(repetition, "repetition", torch.float32, per),
-        ptr(frequency, "frequency", torch.float32, per),
-        ptr(presence, "presence", torch.float32, per),
-        None if bias_ids is None else _dev(bias_ids, "bias_ids", torch.int32).data_ptr(),
-        None if bias_ids is None else _dev(bias, "bias", torch.float32).data_ptr(),
-        None if bias_ids is None else ptr(bias_start, "bias_start", torch.int32, ends),
-        None if allowed is None else allowed.data_ptr(),
-        0 if allowed is None else allowed.shape[1],
-        None if workspace is None else workspace.data_ptr(),
-        0 if workspace is None else workspace.numel() * workspace.element_size(),
-        _stream(logits)))
+        out.data_ptr(), ostride[0], ptr(pick, "pick", i32, rows), logits.data_ptr(), stride[0],
+        rows, n, None if history is None else ptr(history, "history", i32, history.numel()),
+        ptr(history_start, "history_start", i32, rows + 1),
+        ptr(prompt_lens, "prompt_lens", i32, rows), ptr(repetition, "repetition", f32, rows),
+        ptr(frequency, "frequency", f32, rows), ptr(presence, "presence", f32, rows),
+        ptr(bias_ids, "bias_ids", i32, entries),
+        None if bias_ids is None else ptr(bias, "bias", f32, entries),
+        None if bias_ids is None else ptr(bias_start, "bias_start", i32, rows + 1),
+        None if allowed is None else allowed.data_ptr(), words, ws, ws_bytes, _raw_stream(dev)))
     return out, pick
+
+
+@functools.lru_cache(maxsize=1024)
+def _logits_workspace(rows: int, n: int) -> int:
+    return int(lib().rkv_process_logits_workspace_bytes(rows, n))
 
 
 def embed(table: torch.Tensor, ids: torch.Tensor, pe: torch.Tensor | None = None,
