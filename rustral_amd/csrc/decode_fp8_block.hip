@@ -1,4 +1,5 @@
-// decode_fp8_block.hip -- the decode kernels over fp8 pools (v_mfma_f32_16x16x32_bf16).
+// decode_fp8_block.hip -- the decode kernels over fp8 pools with one scale a tile
+// (v_mfma_f32_16x16x32_bf16).
 #include "decode_stream.hpp"
 
 namespace rkv {

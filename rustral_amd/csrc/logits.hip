@@ -105,16 +105,15 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(LogitsArgs p) 
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int c = id[u] - c0;
-        if (id[u] >= 0 && (uint32_t)c < (uint32_t)cols) {
-          if (at + tid + kThreads * u < made) atomicOr(&s_count[c], kPrompt);
-          else atomicAdd(&s_count[c], 1u);
+        if (id[u] >= c0 && id[u] - c0 < cols) {
+          if (at + tid + kThreads * u < made) atomicOr(&s_count[id[u] - c0], kPrompt);
+          else atomicAdd(&s_count[id[u] - c0], 1u);
         }
       }
     }
     for (int i = b0 + tid; i < b1; i += kThreads) {
-      const int c = p.bias_ids[i] - c0;
-      if ((uint32_t)c < (uint32_t)cols) atomicMax(&s_bias[c], (uint32_t)(i - b0) + 1u);
+      const int id = p.bias_ids[i];
+      if (id >= c0 && id - c0 < cols) atomicMax(&s_bias[id - c0], (uint32_t)(i - b0) + 1u);
     }
     __syncthreads();
   }

@@ -1,5 +1,5 @@
 // paged_prefill.hip -- causal prefill attention over fp32 and bf16 pools
-// (rkv_prefill_attention): the builds of the MFMA kernel of prefill_kernel.hpp, and
+// (rkv_prefill_attention): the builds of the mfma kernel of prefill_kernel.hpp, and
 // which one a call takes.
 #include "prefill_kernel.hpp"
 
@@ -104,7 +104,7 @@ extern "C" int rkv_prefill_attention(float* out, const float* q, const void* k_p
   // as slots free up.  The touches go to the last min(R, T - R) workgroups
   // of the first round (its lightest: the grid runs heaviest first), each
   // for the workgroup that many places later; the heaviest, which end the
-  // first round, touch nothing.  configs[4] admissions (us per call, one
+  // first round, touch nothing.  25 admissions of a serving step (us per call, one
   // box, interleaved): 26.7 against 28.6 when the first T - R workgroups
   // touch and 27.4 when the first R - (T - R) touch workgroups of the first
   // round (8 x 512 square: the same workgroups either way, 52.6).

@@ -1,6 +1,6 @@
 // paged_prefill_q.hip -- causal prefill attention over 8-bit pools with one scale
-// a tile (rkv_prefill_attention_q): the MFMA kernel of prefill_kernel.hpp, whose
-// tiles become bf16 as they are staged.
+// a tile (rkv_prefill_attention_q): the mfma kernel of prefill_kernel.hpp, whose
+// tiles become fp16 as they are staged.
 #include "block_quant.hpp"
 #include "prefill_kernel.hpp"
 

@@ -30,13 +30,20 @@
 //     exactly the S^T layout above (no cross-lane moves); P is split hi + lo
 //     like q.  Result: lane l holds O^T[dim 16c + 4(l/16)+r][row l%16].
 // fp32 pools split K and V into hi + lo bf16 as well (three products each).
-// 8-bit pools: the bytes become bf16 on their way into LDS (exact: at most 8
-// significant bits), so everything behind the staging is the bf16 kernel's.  An
-// e4m3 tile's scale is a power of two and goes into that conversion, exactly; an
-// int8 tile's K scale multiplies its scores (16 keys, one MFMA result, wave-
-// uniform) and its V scale the softmax weights.  V rows past the workgroup's last
-// query and of invalid blocks are staged as zeros: their bytes are whatever the
-// memory held, a NaN among them, and a zero weight does not clear a NaN.
+// 8-bit pools with one scale a tile: bytes become fp16 on their way into LDS (exact:
+// int8 integers and e4m3 values fit its 11 bits), and the products run on
+// v_mfma_f32_16x16x32_f16, whose hi + lo terms carry 22 bits where bf16's carry 16,
+// at the same rate.  fp16's range is kept by factors:
+//   * a query row enters as q 2^-E with its largest element in [2^12, 2^13); a
+//     tile's scores are multiplied by its K scale and 2^E (16 keys, one MFMA
+//     result) as they become relative to the reference maximum;
+//   * softmax weights (at most 2^8) enter times V scale / R, R a reference that
+//     starts at the first tile's V scale / 64 and moves, with a rescale of the
+//     accumulators, only for a tile of more than 128 R: products stay under 2^15,
+//     and what is below 2^-31 of the largest V scale's weights is rounded off.
+// V rows past the workgroup's last query and of invalid blocks are staged as zeros:
+// their bytes are whatever the memory held, a NaN among them, and a zero weight
+// does not clear a NaN.
 // MFMA lane layouts (gfx950): 16x16x32: A[l%16][8(l/16)+e], B[8(l/16)+e][l%16];
 // 16x16x16: A[l%16][4(l/16)+e], B[4(l/16)+e][l%16]; both D[4(l/16)+r][l%16].
 #pragma once
@@ -86,25 +93,57 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = cvt_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
 }
 
-// 8 stored bytes (two dwords) as 8 packed bf16: e4m3 times the tile's power of two
-// (v_cvt_scalef32_pk_bf16_fp8 takes the factor as it converts), int8 as they are.
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+
+// The same in fp16: hi truncated (v_cvt_pkrtz_f16_f32, one instruction a pair; the
+// remainder takes what it left), lo from the exact remainder.
+__device__ __forceinline__ void split2h(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+  const f16x2_t hv = __builtin_bit_cast(f16x2_t, h);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(
+      uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hv[0], -1.0f, a), fmaf((float)hv[1], -1.0f, b)));
+}
+
+// bf16 or fp16 terms, and the product that takes them.
+template <bool F16>
+__device__ __forceinline__ void split_term(float a, float b, uint32_t& hi, uint32_t& lo) {
+  if constexpr (F16) split2h(a, b, hi, lo);
+  else split2(a, b, hi, lo);
+}
+template <bool F16>
+__device__ __forceinline__ f32x4_t mma(const uint4& a, const uint4& b, const f32x4_t& c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// 4 stored bytes as 4 fp16.  e4m3: v_cvt_scalef32_pk_f16_fp8 at scale 1.  int8: the
+// byte with its sign bit flipped is 0 .. 255, which under the exponent of 1024 is
+// 1024 + byte + 128, and 1152 comes off exactly.
 template <int FORMAT>
-__device__ __forceinline__ uint4 widen8(uint32_t lo, uint32_t hi, float s) {
+__device__ __forceinline__ uint2 widen4(uint32_t w) {
   if constexpr (FORMAT == RKV_FP8_BLOCK) {
-    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-    const bf16x2_t a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, false);
-    const bf16x2_t a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, true);
-    const bf16x2_t b0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, false);
-    const bf16x2_t b1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, true);
-    return make_uint4(__builtin_bit_cast(uint32_t, a0), __builtin_bit_cast(uint32_t, a1),
-                      __builtin_bit_cast(uint32_t, b0), __builtin_bit_cast(uint32_t, b1));
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
   } else {
-    const auto two = [](uint32_t w, int e) __attribute__((always_inline)) {
-      return cvt_bf16x2((float)((int32_t)(w << (24 - 8 * e)) >> 24),
-                        (float)((int32_t)(w << (16 - 8 * e)) >> 24));
-    };
-    return make_uint4(two(lo, 0), two(lo, 2), two(hi, 0), two(hi, 2));
+    const uint32_t u = w ^ 0x80808080u;
+    const f16x2_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    // v_perm_b32: selector bytes 0 .. 3 name bytes of u, 4 .. 7 of the constant
+    const f16x2_t a = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+    const f16x2_t b = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+    return make_uint2(__builtin_bit_cast(uint32_t, a + off), __builtin_bit_cast(uint32_t, b + off));
   }
+}
+template <int FORMAT>
+__device__ __forceinline__ uint4 widen8(uint32_t lo, uint32_t hi) {
+  const uint2 a = widen4<FORMAT>(lo), b = widen4<FORMAT>(hi);
+  return make_uint4(a.x, a.y, b.x, b.y);
 }
 
 template <typename T, int D, int G, int HW, int QS, int KB, bool PFN, int FORMAT>
@@ -117,8 +156,8 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
     const float* __restrict__ k_scale, const float* __restrict__ v_scale) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr bool Q8 = sizeof(T) == 1;
-  constexpr bool QI8 = FORMAT == RKV_I8_BLOCK;  // int8: scales beside the products
   static_assert(Q8 == (FORMAT == RKV_I8_BLOCK || FORMAT == RKV_FP8_BLOCK), "8-bit formats");
+  static_assert(!Q8 || KB % 2 == 0, "8-bit tiles go in pairs");
   static_assert(G % HW == 0, "heads per wave must divide the group");
   constexpr int NT = 64 * (G / HW) * QS;
   constexpr int QT = 16 * QS;              // query tokens per workgroup
@@ -129,7 +168,13 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
   constexpr int CE = 16 / sizeof(T);       // elements per 16-byte chunk
   constexpr int CPR = D / CE;              // chunks per token row
   constexpr int CH = kBS * CPR;            // chunks per (block, head) tile
-  constexpr int PT = (KB * CH + NT - 1) / NT;  // chunks per thread and iteration
+  // 8-bit pools are staged in units of 8 bytes: a lane's 8 elements are one 16-byte
+  // LDS store and the lanes' stores contiguous (16 bytes a lane would be two stores 32
+  // bytes apart, which use half the banks).
+  constexpr int UPR = D / 8, UT = kBS * UPR;   // 8-byte units a row, a tile
+  // chunks per thread and iteration: of K and of V, or of the two together in units,
+  // K's first, so that all threads take part
+  constexpr int PT = ((Q8 ? 2 * KB * UT : KB * CH) + NT - 1) / NT;
   constexpr int NC = D / 32;               // QK^T MFMAs per key block (per slice)
   constexpr int NO = D / 16;               // PV MFMAs per key block (per slice)
   // The output rows go out through LDS: each wave writes one head's 16 rows
@@ -138,7 +183,7 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
   // back whole, 512 contiguous bytes per half-wave, where the MFMA layout
   // stored 16 rows x 64 bytes per instruction.  The rows sit after the K/V
   // staging buffers, so no workgroup barrier separates them from the loop.
-  // configs[4] admissions (us per call, one box, one process): 30.5 with
+  // 25 admissions of a serving step (us per call, one box, one process): 30.5 with
   // stores from the MFMA layout, 28.0 through the rows; q staged the same
   // way as well 30.0 (its LDS round trip costs more than the contiguous
   // loads save), both heads' rows at once behind a workgroup barrier 28.7.
@@ -226,6 +271,22 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
         vs[kb] = ok ? c : 0.0f;
       }
     }
+    if constexpr (Q8) {
+#pragma unroll
+      for (int i = 0; i < PT; ++i) {
+        const int ui = tid + i * NT;
+        if ((2 * KB * UT) % NT == 0 || ui < 2 * KB * UT) {
+          const int kb = ui / UT % KB, uu = ui % UT;
+          int64_t bb = base[0];
+#pragma unroll
+          for (int x = 1; x < KB; ++x) bb = kb == x ? base[x] : bb;
+          const u32x2_t v =
+              *reinterpret_cast<const u32x2_t*>((ui < KB * UT ? k_pool : v_pool) + bb + uu * 8);
+          kr[i].x = v.x, kr[i].y = v.y;
+        }
+      }
+      return okm;
+    }
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int ci = tid + i * NT;
@@ -241,8 +302,26 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
     return okm;
   };
   // Writes the registers into LDS buffer buf (K and V row-major).
-  auto stage = [&](int it, int buf, uint32_t okm, const u32x4_t (&kr)[PT], const u32x4_t (&vr)[PT],
-                   const float (&ks)[KB], const float (&vs)[KB]) __attribute__((always_inline)) {
+  auto stage = [&](int it, int buf, uint32_t okm, const u32x4_t (&kr)[PT],
+                   const u32x4_t (&vr)[PT]) __attribute__((always_inline)) {
+    if constexpr (Q8) {
+#pragma unroll
+      for (int i = 0; i < PT; ++i) {
+        const int ui = tid + i * NT;
+        if ((2 * KB * UT) % NT == 0 || ui < 2 * KB * UT) {
+          const int kb = ui / UT % KB, uu = ui % UT;
+          const int key = uu / UPR, col = (uu % UPR) * 8;
+          const bool is_k = ui < KB * UT;
+          const bool held =
+              is_k || (((okm >> kb) & 1u) && (it * KB + kb) * kBS + key <= last);
+          uint16_t* to = is_k ? &s_k[buf][0][(kb * kBS + key) * KP + col]
+                              : &s_v[buf][0][(kb * kBS + key) * VKP + col];
+          *reinterpret_cast<uint4*>(to) =
+              widen8<FORMAT>(held ? kr[i].x : 0u, held ? kr[i].y : 0u);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int ci = tid + i * NT;
@@ -251,19 +330,7 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
         const int key = cc / CPR, col = (cc % CPR) * CE;
         uint16_t* kd = &s_k[buf][0][(kb * kBS + key) * KP + col];
         uint16_t* vd = &s_v[buf][0][(kb * kBS + key) * VKP + col];
-        if constexpr (Q8) {
-          float kq = ks[0], vq = vs[0];  // ks[kb] by selects
-#pragma unroll
-          for (int x = 1; x < KB; ++x) kq = kb == x ? ks[x] : kq, vq = kb == x ? vs[x] : vq;
-          const bool held = ((okm >> kb) & 1u) && (it * KB + kb) * kBS + key <= last;
-          u32x4_t vz = vr[i];
-          vz.x = held ? vz.x : 0u, vz.y = held ? vz.y : 0u;
-          vz.z = held ? vz.z : 0u, vz.w = held ? vz.w : 0u;
-          *reinterpret_cast<uint4*>(kd) = widen8<FORMAT>(kr[i].x, kr[i].y, kq);
-          *reinterpret_cast<uint4*>(kd + 8) = widen8<FORMAT>(kr[i].z, kr[i].w, kq);
-          *reinterpret_cast<uint4*>(vd) = widen8<FORMAT>(vz.x, vz.y, vq);
-          *reinterpret_cast<uint4*>(vd + 8) = widen8<FORMAT>(vz.z, vz.w, vq);
-        } else if constexpr (!F32) {
+        if constexpr (!F32) {
           *reinterpret_cast<u32x4_t*>(kd) = kr[i];
           *reinterpret_cast<u32x4_t*>(vd) = vr[i];
         } else {
@@ -317,20 +384,44 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
   // B operand of S^T = K Q^T: Q[row r16][32c + 8 grp .. + 8] * q_scale, hi
   // and lo (scores come out already scaled by scale * log2 e), converted
   // from the raw rows loaded before the first K/V fetch.
+  // 8-bit pools: the row's power of two comes off first (rowf puts it back).
   uint4 qhi[HW][NC], qlo[HW][NC];
+  float rowf[HW];
 #pragma unroll
-  for (int hh = 0; hh < HW; ++hh)
+  for (int hh = 0; hh < HW; ++hh) {
+    float down = 1.0f;
+    if constexpr (Q8) {
+      float top = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float4 x = qraw[hh][c][0], y = qraw[hh][c][1];
+        top = fmaxf(top, fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                               fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
+      }
+      top = xor48_max(top * fabsf(q_scale));  // of the row
+      // 2^(12 - exponent of top), within 2^-100 .. 2^100 (a zero row, an infinity)
+      int e = 139 - (int)(__float_as_uint(top) >> 23);
+      e = e < -100 ? -100 : (e > 100 ? 100 : e);
+      down = __uint_as_float((uint32_t)(127 + e) << 23);
+      rowf[hh] = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float4 x = qraw[hh][c][0], y = qraw[hh][c][1];
       if (!row_ok) x = y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       x.x *= q_scale; x.y *= q_scale; x.z *= q_scale; x.w *= q_scale;
       y.x *= q_scale; y.y *= q_scale; y.z *= q_scale; y.w *= q_scale;
-      split2(x.x, x.y, qhi[hh][c].x, qlo[hh][c].x);
-      split2(x.z, x.w, qhi[hh][c].y, qlo[hh][c].y);
-      split2(y.x, y.y, qhi[hh][c].z, qlo[hh][c].z);
-      split2(y.z, y.w, qhi[hh][c].w, qlo[hh][c].w);
+      if constexpr (Q8) {
+        x.x *= down; x.y *= down; x.z *= down; x.w *= down;
+        y.x *= down; y.y *= down; y.z *= down; y.w *= down;
+      }
+      split_term<Q8>(x.x, x.y, qhi[hh][c].x, qlo[hh][c].x);
+      split_term<Q8>(x.z, x.w, qhi[hh][c].y, qlo[hh][c].y);
+      split_term<Q8>(y.x, y.y, qhi[hh][c].z, qlo[hh][c].z);
+      split_term<Q8>(y.z, y.w, qhi[hh][c].w, qlo[hh][c].w);
     }
+  }
+  float vref = 0.0f, vinv = 0.0f;  // the row's V scale reference R and 1 / R
 
   f32x4_t o[HW][NO];
   float m[HW], l[HW];
@@ -403,7 +494,7 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
       f32x4_t st[HW];
 #pragma unroll
       for (int hh = 0; hh < HW; ++hh) {
-        const float from = QI8 ? 0.0f : -mref[hh];  // int8: the tile's scale comes in between
+        const float from = Q8 ? 0.0f : -mref[hh];  // 8-bit: the tile's scale comes in between
         st[hh] = f32x4_t{from, from, from, from};
       }
       const uint16_t* kr0 = &s_k[buf][0][(kb * kBS + r16) * KP + 8 * grp];
@@ -411,15 +502,9 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
       for (int c = 0; c < NC; ++c) {
         const uint4 ka = *reinterpret_cast<const uint4*>(kr0 + 32 * c);
 #pragma unroll
-        for (int hh = 0; hh < HW; ++hh)
-          st[hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8_t, ka), __builtin_bit_cast(bf16x8_t, qhi[hh][c]), st[hh],
-              0, 0, 0);
+        for (int hh = 0; hh < HW; ++hh) st[hh] = mma<Q8>(ka, qhi[hh][c], st[hh]);
 #pragma unroll
-        for (int hh = 0; hh < HW; ++hh)
-          st[hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8_t, ka), __builtin_bit_cast(bf16x8_t, qlo[hh][c]), st[hh],
-              0, 0, 0);
+        for (int hh = 0; hh < HW; ++hh) st[hh] = mma<Q8>(ka, qlo[hh][c], st[hh]);
         if constexpr (F32) {
           const uint4 kl =
               *reinterpret_cast<const uint4*>(kr0 + KB * kBS * KP + 32 * c);
@@ -430,11 +515,13 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
                 st[hh], 0, 0, 0);
         }
       }
-      if constexpr (QI8) {
+      if constexpr (Q8) {
 #pragma unroll
-        for (int hh = 0; hh < HW; ++hh)
+        for (int hh = 0; hh < HW; ++hh) {
+          const float f = ks[kb] * rowf[hh];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) st[hh][r] = fmaf(st[hh][r], ks[kb], -mref[hh]);
+          for (int r = 0; r < 4; ++r) st[hh][r] = fmaf(st[hh][r], f, -mref[hh]);
+        }
       }
       if constexpr (MASKED) {
         // causal mask: key 4 grp + r of the block is kept when r <= lim
@@ -472,7 +559,22 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
       // before the row's first key (m = -inf) any key moves m
       up = up || mb > (m[hh] == -INFINITY ? -INFINITY : kSlack);
     }
-    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+    // 8-bit pools: the V scales' reference, of the row's own tiles (one behind its
+    // last key could be anything), moves in the same branch
+    bool vmove = false;
+    float vto = vref, vsr[KB];
+    if constexpr (Q8) {
+      float top = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        vsr[kb] = !MASKED || kfirst + kb * kBS <= qpos ? vs[kb] : 0.0f;
+        top = fmaxf(top, vsr[kb]);
+      }
+      vmove = top > 128.0f * vref;  // the first tile, and rarely another
+      vto = vmove ? top * 0.015625f : vref;
+    }
+    if (__builtin_amdgcn_ballot_w64(up || vmove) != 0) {
+      const float vratio = Q8 && vmove ? vref / vto : 1.0f;
 #pragma unroll
       for (int hh = 0; hh < HW; ++hh) {
         const float mx = xor48_max(lm[hh]);  // the row's maximum, relative to mref
@@ -484,7 +586,7 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
 #pragma unroll
         for (int c = 0; c < NO; ++c)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[hh][c][r] *= alpha;
+          for (int r = 0; r < 4; ++r) o[hh][c][r] *= Q8 ? alpha * vratio : alpha;
         m[hh] = mn;
         const float d = mref_new - mref[hh];  // the scores move to the new reference
 #pragma unroll
@@ -492,6 +594,8 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[hh][kb][r] -= d;
       }
+      if constexpr (Q8)
+        if (vmove) vref = vto, vinv = 1.0f / vto;
     }
 #pragma unroll
     for (int hh = 0; hh < HW; ++hh) {
@@ -506,13 +610,15 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
         }
       l[hh] += ls;  // this lane's keys of the row; the row's lanes are summed at the end
     }
-    if constexpr (QI8) {
+    if constexpr (Q8) {
 #pragma unroll
-      for (int hh = 0; hh < HW; ++hh)
+      for (int kb = 0; kb < KB; ++kb) {
+        const float f = vsr[kb] * vinv;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+        for (int hh = 0; hh < HW; ++hh)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[hh][kb][r] *= vs[kb];
+          for (int r = 0; r < 4; ++r) s[hh][kb][r] *= f;
+      }
     }
 
     // ---- O^T += V^T P^T ----
@@ -526,10 +632,10 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
         uint4 ph[HW], pl[HW];
 #pragma unroll
         for (int hh = 0; hh < HW; ++hh) {
-          split2(s[hh][kb][0], s[hh][kb][1], ph[hh].x, pl[hh].x);
-          split2(s[hh][kb][2], s[hh][kb][3], ph[hh].y, pl[hh].y);
-          split2(s[hh][kb + 1][0], s[hh][kb + 1][1], ph[hh].z, pl[hh].z);
-          split2(s[hh][kb + 1][2], s[hh][kb + 1][3], ph[hh].w, pl[hh].w);
+          split_term<Q8>(s[hh][kb][0], s[hh][kb][1], ph[hh].x, pl[hh].x);
+          split_term<Q8>(s[hh][kb][2], s[hh][kb][3], ph[hh].y, pl[hh].y);
+          split_term<Q8>(s[hh][kb + 1][0], s[hh][kb + 1][1], ph[hh].z, pl[hh].z);
+          split_term<Q8>(s[hh][kb + 1][2], s[hh][kb + 1][3], ph[hh].w, pl[hh].w);
         }
         // this lane's transposing-read address: key 4 grp + (r16 >> 2),
         // dims 16 c + 4 (r16 & 3) .. + 3
@@ -541,15 +647,9 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
           const uint2 a1 = lds_read_tr16(va1 + 16 * c);
           const uint4 va = make_uint4(a0.x, a0.y, a1.x, a1.y);
 #pragma unroll
-          for (int hh = 0; hh < HW; ++hh)
-            o[hh][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, va), __builtin_bit_cast(bf16x8_t, ph[hh]), o[hh][c],
-                0, 0, 0);
+          for (int hh = 0; hh < HW; ++hh) o[hh][c] = mma<Q8>(va, ph[hh], o[hh][c]);
 #pragma unroll
-          for (int hh = 0; hh < HW; ++hh)
-            o[hh][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, va), __builtin_bit_cast(bf16x8_t, pl[hh]), o[hh][c],
-                0, 0, 0);
+          for (int hh = 0; hh < HW; ++hh) o[hh][c] = mma<Q8>(va, pl[hh], o[hh][c]);
           if constexpr (F32) {
             const uint2 l0 = lds_read_tr16(va0 + KB * kBS * VKP + 16 * c);
             const uint2 l1 = lds_read_tr16(va1 + KB * kBS * VKP + 16 * c);
@@ -608,18 +708,18 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
   // bodies free of exits between the two halves.
   auto pair = [&](auto masked, int it) __attribute__((always_inline)) {
     float ksc[KB], vsc[KB];  // the staged tiles' scales
-    stage(it, 0, ok0, kr0, vr0, ks0, vs0);
+    stage(it, 0, ok0, kr0, vr0);
     const uint32_t okA = ok0;
-    if constexpr (QI8)
+    if constexpr (Q8)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) ksc[kb] = ks0[kb], vsc[kb] = vs0[kb];
     __syncthreads();
     ok0 = fetch(ids, kr0, vr0, ks0, vs0);
     load_ids(it + 3, ids);
     step(masked, it, 0, okA, ksc, vsc);
-    stage(it + 1, 1, ok1, kr1, vr1, ks1, vs1);
+    stage(it + 1, 1, ok1, kr1, vr1);
     const uint32_t okB = ok1;
-    if constexpr (QI8)
+    if constexpr (Q8)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) ksc[kb] = ks1[kb], vsc[kb] = vs1[kb];
     __syncthreads();
@@ -653,7 +753,7 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
     if (!row_ok) return;
 #pragma unroll
     for (int hh = 0; hh < HW; ++hh) {
-      const float inv = l[hh] > 0.0f ? 1.0f / l[hh] : 0.0f;
+      const float inv = l[hh] > 0.0f ? (Q8 ? vref : 1.0f) / l[hh] : 0.0f;
       float* op = out + ((int64_t)(s0 + qi) * num_q_heads + h0 + hh) * D + 4 * grp;
 #pragma unroll
       for (int c = 0; c < NO; ++c)
@@ -677,7 +777,7 @@ __global__ __launch_bounds__(64 * (G / HW) * QS) __attribute__((amdgpu_waves_per
     float* orows = reinterpret_cast<float*>(s_raw + KV_BYTES) + w * 16 * RWO;
 #pragma unroll
     for (int hh = 0; hh < HW; ++hh) {
-      const float inv = l[hh] > 0.0f ? 1.0f / l[hh] : 0.0f;
+      const float inv = l[hh] > 0.0f ? (Q8 ? vref : 1.0f) / l[hh] : 0.0f;
 #pragma unroll
       for (int c = 0; c < NO; ++c)
         *reinterpret_cast<float4*>(orows + r16 * RWO + 16 * c + 4 * grp) =
@@ -773,7 +873,7 @@ struct PrefillCfg {
 // Workgroups of fn (threads each) resident on the current device at once:
 // compute units x workgroups per compute unit, asked of the runtime once per
 // (device, kernel) and kept; 0 if the runtime cannot say.
-int resident_workgroups(PrefillFn fn, int threads) {
+[[maybe_unused]] int resident_workgroups(PrefillFn fn, int threads) {
   struct Entry {
     PrefillFn fn;
     int device, resident;

@@ -295,3 +295,29 @@ def test_block_front_end_refuses(dev):
         kv.decode_attention_append_q(q, k, k, s, s, x[:1], x[:1], tab, ctx, None, "int8_block")
     with pytest.raises(_lib.RkvError):
         kv.prefill_attention_q(torch.zeros((3, 6, 64), device=dev), k, k, s, s, tab, st, ctx)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 2.0 ** 100])
+def test_prefill_rows_before_a_tile_do_not_see_its_scales(dev, fmt, bad):
+    """The tile of positions 32 .. 47 gets scales of NaN, infinity or 2^100: the rows
+    before it keep every bit, whichever wave and iteration they share with it."""
+    say(f"prefill before a bad tile {fmt} {bad}")
+    rng = np.random.default_rng(9)
+    for ctx0, hq, hkv, d in [(40, 8, 2, 128), (70, 8, 8, 64), (48, 8, 1, 128)]:
+        for cached in (0, 10, 27):
+            n, ctx = np.array([ctx0 - cached], np.int32), np.array([ctx0], np.int32)
+            nb = 6
+            tables = make_tables(rng, ctx, 16, nb)
+            k, v, ks, vs = filled(rng, nb, hkv, d, fmt, 0.5)
+            q = rng.standard_normal((int(n[0]), hq, d)).astype(np.float32)
+            outs = []
+            for scale in (None, bad):
+                if scale is not None:
+                    ks[tables[0, 2]], vs[tables[0, 2]] = scale, scale
+                g = [to_dev(a, dev) for a in (k, v, ks, vs, tables, np.array([0, n[0]], np.int32),
+                                              ctx)]
+                outs.append(to_np(kv.prefill_attention_q(to_dev(q, dev), *g, None, fmt)))
+            rows = 32 - cached
+            assert np.isfinite(outs[1][:rows]).all()
+            assert np.array_equal(outs[0][:rows], outs[1][:rows]), (ctx0, cached)
