@@ -109,24 +109,26 @@ __device__ __forceinline__ uint32_t tile_word(const float4& x, float s, float in
 template <int DT>
 __device__ __forceinline__ uint32_t tile_reword(uint32_t w, float s_old, float s, float ratio) {
   if constexpr (DT == RKV_I8_BLOCK) {
-    float r[4];
-    bool near = false;
+    // byte + 128 converts in one instruction, and 128 * ratio comes off in the
+    // product's rounding; adding 1.5 * 2^23 leaves the rounded integer in the low byte
+    constexpr float kMagic = 12582912.0f;
+    const uint32_t u = w ^ 0x80808080u;
+    float z[4], far = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float y = (float)((int32_t)(w << (24 - 8 * e)) >> 24) * ratio;
-      r[e] = rintf(y);
-      near = near || near_middle(y, r[e]);
+      const float y = fmaf((float)((u >> (8 * e)) & 0xffu), ratio, -128.0f * ratio);
+      z[e] = y + kMagic;
+      far = fmaxf(far, fabsf(y - (z[e] - kMagic)));
     }
-    if (near) {
+    if (far > 0.4999f) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        r[e] = exact_round(r[e], (double)((int32_t)(w << (24 - 8 * e)) >> 24) * (double)s_old,
-                           (double)s);
+        z[e] = kMagic + exact_round(z[e] - kMagic, (double)((int32_t)(w << (24 - 8 * e)) >> 24) *
+                                                       (double)s_old, (double)s);
     }
-    uint32_t o = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o |= ((uint32_t)(int)r[e] & 0xffu) << (8 * e);
-    return o;
+    const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(z[1]), __float_as_uint(z[0]), 0x0c0c0400u);
+    const uint32_t c = __builtin_amdgcn_perm(__float_as_uint(z[3]), __float_as_uint(z[2]), 0x04000c0cu);
+    return a | c;
   } else {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
     const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
