@@ -35,6 +35,19 @@ def _stream(t: torch.Tensor) -> int:
     return _raw_stream(t.get_device())
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _launch(dev: int, fn, *args) -> None:
+    """fn(*args, stream) on device dev's current stream, with dev the current device
+    meanwhile: the default stream's handle, 0, means the current device's."""
+    if dev == _current_device():
+        check(fn(*args, _raw_stream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _raw_stream(dev)))
+
+
 def _dev(t: torch.Tensor, name: str, dtype=None) -> torch.Tensor:
     if t.is_cuda and (dtype is None or t.dtype is dtype) and t.is_contiguous():
         return t
@@ -52,6 +65,13 @@ def _one_device(dev: int, named) -> None:
     for t, name in named:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{name} must be on the call's device")
+
+
+def _out_like(out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
+    _dev(out, "out", torch.float32)
+    if out.shape != q.shape or out.get_device() != q.get_device():
+        raise ValueError("out must have q's shape, on its device")
+    return out
 
 
 def check_attention_shapes(q_shape, pool_shape, tables_shape, lens_shape,
@@ -493,11 +513,10 @@ def decode_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     ws_ptr = workspace.data_ptr() if workspace is not None else None
     ws_len = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    check(lib().rkv_decode_attention_q(out.data_ptr(), q.data_ptr(), k_pool.data_ptr(),
-                                       v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                       block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, hq,
-                                       hkv, d, bs, nb, max_context, float(scale), code,
-                                       partition_size, ws_ptr, ws_len, _raw_stream(dev)))
+    _launch(dev, lib().rkv_decode_attention_q, out.data_ptr(), q.data_ptr(), k_pool.data_ptr(),
+            v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+            mbs, ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, max_context, float(scale), code,
+            partition_size, ws_ptr, ws_len)
     return out
 
 
@@ -585,12 +604,11 @@ def append_block_q(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Te
         raise ValueError("one block-table row and one length per sequence, new_start B + 1 offsets")
     if max_new is None:
         max_new = int((new_start[1:] - new_start[:-1]).max().item()) if B else 0
-    check(lib().rkv_append_block_q(
-        k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-        nb * hkv * bs * d if multi else 0, k_new.data_ptr(), v_new.data_ptr(),
-        total * hkv * d if multi else 0, hkv * d, d, new_start.data_ptr(),
-        block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, n_layers, hkv, d, bs, nb, max_new,
-        code, _raw_stream(dev)))
+    _launch(dev, lib().rkv_append_block_q, k_pool.data_ptr(), v_pool.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), nb * hkv * bs * d if multi else 0,
+            k_new.data_ptr(), v_new.data_ptr(), total * hkv * d if multi else 0, hkv * d, d,
+            new_start.data_ptr(), block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, n_layers,
+            hkv, d, bs, nb, max_new, code)
 
 
 def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -619,11 +637,12 @@ def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         scale = 1.0 / math.sqrt(d)
     if out is None:
         out = torch.zeros_like(q)
-    check(lib().rkv_prefill_attention_q(
-        out.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
-        ctx_lens.data_ptr(), B, q.shape[1], hkv, d, bs, nb, max_q_len, float(scale), code,
-        _stream(q)))
+    else:
+        _out_like(out, q)
+    _launch(q.get_device(), lib().rkv_prefill_attention_q, out.data_ptr(), q.data_ptr(),
+            k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
+            ctx_lens.data_ptr(), B, q.shape[1], hkv, d, bs, nb, max_q_len, float(scale), code)
     return out
 
 
@@ -688,9 +707,9 @@ def rope(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *,
     elif _rows(out, "out").shape != x.shape or out.get_device() != x.get_device():
         raise ValueError("out must have x's shape, on its device")
     t, h, d = x.shape
-    check(lib().rkv_rope(out.data_ptr(), x.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
-                         t, h, d, 2 * inv_freq.shape[0], out.stride(0), out.stride(1),
-                         x.stride(0), x.stride(1), int(interleaved), magnitude, _stream(x)))
+    _launch(x.get_device(), lib().rkv_rope, out.data_ptr(), x.data_ptr(), positions.data_ptr(),
+            inv_freq.data_ptr(), t, h, d, 2 * inv_freq.shape[0], out.stride(0), out.stride(1),
+            x.stride(0), x.stride(1), int(interleaved), magnitude)
     return out
 
 
@@ -730,7 +749,7 @@ def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     if nshape != (t, hkv, d) or v_new.shape != nshape or dq != d:
         raise ValueError(f"q {tuple(qshape)}, k_new {tuple(nshape)}, v_new "
                          f"{tuple(v_new.shape)} do not match pool {tuple(shape)}")
-    if ns != vs_:
+    if ns != vs_ and (t > 1 and ns[0] != vs_[0] or hkv > 1 and ns[1] != vs_[1]):
         raise ValueError("k_new and v_new must have the same strides")
     (half,) = inv_freq.shape
     if positions.shape != (t,) or slot_mapping.shape != (t,) or 2 * half > d:
@@ -753,11 +772,10 @@ def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
         os = out.stride()
         if out.shape != qshape or out.dtype is not f32 or os[-1] != 1 or out.get_device() != dev:
             raise ValueError("out must be fp32 of q's shape with contiguous rows, on its device")
-    check(lib().rkv_rope_append(
-        out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks, vs, q.data_ptr(),
-        k_new.data_ptr(), v_new.data_ptr(), os[0], os[1], qs[0], qs[1], ns[0], ns[1],
-        positions.data_ptr(), inv_freq.data_ptr(), slot_mapping.data_ptr(), t, hq, hkv, d,
-        2 * half, int(interleaved), magnitude, bs, nb, code, _raw_stream(dev)))
+    _launch(dev, lib().rkv_rope_append, out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks,
+            vs, q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), os[0], os[1], qs[0], qs[1],
+            ns[0], ns[1], positions.data_ptr(), inv_freq.data_ptr(), slot_mapping.data_ptr(), t,
+            hq, hkv, d, 2 * half, int(interleaved), magnitude, bs, nb, code)
     return out
 
 
@@ -813,14 +831,17 @@ def decode_attention_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
         scale = 1.0 / math.sqrt(d)
     if out is None:
         out = torch.empty_like(q)
-    if workspace is None:  # a caller's is checked by the library
+    else:
+        _out_like(out, q)
+    if workspace is None:  # the library checks the size of a caller's
         need = weights_workspace_bytes(B, hq, hkv, d, max_context)
         workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-    check(lib().rkv_decode_attention_weights(
-        out.data_ptr(), weights.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks,
-        vs, block_tables.data_ptr(), mbs, ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, max_context,
-        float(scale), code, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        _stream(q)))
+    else:
+        _one_device(q.get_device(), ((_dev(workspace, "workspace"), "workspace"),))
+    _launch(q.get_device(), lib().rkv_decode_attention_weights, out.data_ptr(), weights.data_ptr(),
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks, vs, block_tables.data_ptr(),
+            mbs, ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, max_context, float(scale), code,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size())
     return out
 
 
@@ -851,11 +872,10 @@ def evict_select(weights: torch.Tensor, block_tables: torch.Tensor, ctx_lens: to
         new_lens = torch.empty(B, dtype=torch.int32, device=weights.device)
     elif _dev(new_lens, "new_lens", torch.int32).shape != (B,):
         raise ValueError("new_lens must be [B]")
-    check(lib().rkv_evict_select(keep.data_ptr(), new_lens.data_ptr(), weights.data_ptr(),
-                                 nb * hkv * bs, block_tables.data_ptr(), mbs, ctx_lens.data_ptr(),
-                                 B, n_layers, hkv, bs, nb, budget, sinks, recent,
-                                 mbs * bs if max_context is None else max_context,
-                                 _stream(weights)))
+    _launch(weights.get_device(), lib().rkv_evict_select, keep.data_ptr(), new_lens.data_ptr(),
+            weights.data_ptr(), nb * hkv * bs, block_tables.data_ptr(), mbs, ctx_lens.data_ptr(),
+            B, n_layers, hkv, bs, nb, budget, sinks, recent,
+            mbs * bs if max_context is None else max_context)
     return keep, new_lens
 
 
@@ -887,12 +907,11 @@ def evict_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, keep: torch.Tensor
         raise ValueError("one source and one destination table row per sequence")
     if weights is not None and _dev(weights, "weights", torch.float32).shape != k_pool.shape[:-1]:
         raise ValueError("weights must be the pools' shape without head_dim")
-    check(lib().rkv_evict_compact(
-        k_pool.data_ptr(), v_pool.data_ptr(), ks, vs,
-        weights.data_ptr() if weights is not None else None, nb * hkv * bs * d, nb * hkv * bs,
-        keep.data_ptr(), new_lens.data_ptr(), keep.shape[-1], src_tables.data_ptr(),
-        src_tables.shape[1], dst_tables.data_ptr(), dst_tables.shape[1], B, n_layers, hkv, d, bs,
-        nb, code, _stream(k_pool)))
+    _launch(k_pool.get_device(), lib().rkv_evict_compact, k_pool.data_ptr(), v_pool.data_ptr(), ks,
+            vs, weights.data_ptr() if weights is not None else None, nb * hkv * bs * d,
+            nb * hkv * bs, keep.data_ptr(), new_lens.data_ptr(), keep.shape[-1],
+            src_tables.data_ptr(), src_tables.shape[1], dst_tables.data_ptr(), dst_tables.shape[1],
+            B, n_layers, hkv, d, bs, nb, code)
 
 
 class DeviceBlockManager:

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from ._lib import RkvError, check, lib
-from .kv import _dev, _dtype_code, _raw_stream, _stream
+from .kv import _dev, _dtype_code, _launch, _one_device, _stream
 
 
 class DecoderConfig(C.Structure):
@@ -415,6 +415,7 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         pick = torch.empty(rows, dtype=i32, device=logits.device)
     ws_bytes, ws = _logits_workspace(rows, n), None
     if workspace is not None:
+        _one_device(dev, ((_dev(workspace, "workspace"), "workspace"),))
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif ws_bytes:
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
@@ -431,16 +432,16 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
     if bias_ids is not None and (bias is None or bias_start is None):
         raise ValueError("bias_ids needs bias of the same length and bias_start")
     entries = 0 if bias_ids is None else bias_ids.numel()
-    check(lib().rkv_process_logits(
-        out.data_ptr(), ostride[0], ptr(pick, "pick", i32, rows), logits.data_ptr(), stride[0],
-        rows, n, None if history is None else ptr(history, "history", i32, history.numel()),
-        ptr(history_start, "history_start", i32, rows + 1),
-        ptr(prompt_lens, "prompt_lens", i32, rows), ptr(repetition, "repetition", f32, rows),
-        ptr(frequency, "frequency", f32, rows), ptr(presence, "presence", f32, rows),
-        ptr(bias_ids, "bias_ids", i32, entries),
-        None if bias_ids is None else ptr(bias, "bias", f32, entries),
-        None if bias_ids is None else ptr(bias_start, "bias_start", i32, rows + 1),
-        None if allowed is None else allowed.data_ptr(), words, ws, ws_bytes, _raw_stream(dev)))
+    _launch(dev, lib().rkv_process_logits, out.data_ptr(), ostride[0],
+            ptr(pick, "pick", i32, rows), logits.data_ptr(), stride[0], rows, n,
+            None if history is None else ptr(history, "history", i32, history.numel()),
+            ptr(history_start, "history_start", i32, rows + 1),
+            ptr(prompt_lens, "prompt_lens", i32, rows), ptr(repetition, "repetition", f32, rows),
+            ptr(frequency, "frequency", f32, rows), ptr(presence, "presence", f32, rows),
+            ptr(bias_ids, "bias_ids", i32, entries),
+            None if bias_ids is None else ptr(bias, "bias", f32, entries),
+            None if bias_ids is None else ptr(bias_start, "bias_start", i32, rows + 1),
+            None if allowed is None else allowed.data_ptr(), words, ws, ws_bytes)
     return out, pick
 
 

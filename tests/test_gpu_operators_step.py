@@ -286,3 +286,90 @@ def test_two_streams_at_once(dev):
         for run in got[i]:
             for a, b in zip(run, alone[i]):
                 assert torch.equal(a, b)
+
+
+def small(dev):
+    """Tensors of a small call of every entry point, by name, and the calls."""
+    rng = np.random.default_rng(8)
+    lens = np.array([20, 37], np.int32)
+    tables = np.array([[0, 1, -1], [2, 3, 4]], np.int32)
+    t = {n: to_dev(rng.standard_normal(s).astype(np.float32), dev)
+         for n, s in dict(q=(2, HQ, D), kn=(2, HKV, D), vn=(2, HKV, D), x=(2, 5000)).items()}
+    t.update(tab=to_dev(tables, dev), ctx=to_dev(lens, dev), pos=to_dev(lens - 1, dev),
+             dst=to_dev(np.array([[5, 6], [7, 8]], np.int32), dev),
+             start=to_dev(np.array([0, 1, 2], np.int32), dev),
+             slots=to_dev(np.array([19, 4 * 16 + 4], np.int64), dev),
+             k=torch.zeros((9, HKV, 16, D), device=dev), v=torch.zeros((9, HKV, 16, D), device=dev),
+             w=torch.zeros((9, HKV, 16), device=dev))
+    t.update({n: torch.zeros((9, HKV, 16, D), dtype=torch.uint8, device=dev) for n in ("k8", "v8")})
+    t.update({n: torch.zeros((9, HKV), device=dev) for n in ("ks", "vs")})
+    freq, _ = kv.rope_frequencies(D, device=dev)
+
+    def run():
+        a = kv.rope_append(t["q"], t["kn"], t["vn"], t["pos"], freq, t["k"], t["v"], t["slots"])
+        b = kv.rope(t["kn"], t["pos"], freq)
+        q8 = (t["k8"], t["v8"], t["ks"], t["vs"])
+        kv.append_block_q(*q8, b, t["vn"], t["start"], t["tab"], t["ctx"], max_new=1)
+        c = kv.decode_attention_q(t["q"], *q8, t["tab"], t["ctx"], fmt="int8_block")
+        e = kv.prefill_attention_q(t["q"], *q8, t["tab"], t["start"], t["ctx"], max_q_len=1)
+        f = kv.decode_attention_weights(t["q"], t["k"], t["v"], t["w"], t["tab"], t["ctx"])
+        keep, left = kv.evict_select(t["w"], t["tab"], t["ctx"], 18, sinks=1, recent=2)
+        kv.evict_compact(t["k"], t["v"], keep, left, t["tab"], t["dst"], weights=t["w"])
+        y, pick = model.process_logits(t["x"])
+        return [u.clone() for u in (a, b, c, e, f, keep, left, y, pick, t["k"], t["v"], t["w"],
+                                    t["k8"], t["v8"], t["ks"], t["vs"])]
+
+    return t, freq, run
+
+
+def test_on_a_device_that_is_not_current(dev, monkeypatch):
+    """The calls make their tensors' device the current one: seen from another
+    current device (here as far as the front end can tell) the results are the same."""
+    say("another current device")
+    want = small(dev)[2]()
+    seen = []
+    real = torch.cuda.device
+    monkeypatch.setattr(kv, "_current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: seen.append(d) or real(d))
+    got = small(dev)[2]()
+    assert seen == [0] * 9
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_front_end_refuses_outputs_and_workspaces(dev):
+    """Buffers a kernel would write past, or that the device cannot reach."""
+    say("refusals")
+    t, freq, _ = small(dev)
+    q8 = (t["k8"], t["v8"], t["ks"], t["vs"])
+    for bad, err in ((t["q"][:1].clone(), ValueError), (t["q"].double(), TypeError),
+                     (t["q"].cpu(), ValueError)):
+        with pytest.raises(err):
+            kv.prefill_attention_q(t["q"], *q8, t["tab"], t["start"], t["ctx"], max_q_len=1, out=bad)
+        with pytest.raises(err):
+            kv.decode_attention_weights(t["q"], t["k"], t["v"], t["w"], t["tab"], t["ctx"], out=bad)
+        with pytest.raises((ValueError, TypeError)):
+            kv.rope(t["q"], t["pos"], freq, out=bad)
+        with pytest.raises(ValueError):
+            kv.rope_append(t["q"], t["kn"], t["vn"], t["pos"], freq, t["k"], t["v"], t["slots"],
+                           out=bad)
+    host = torch.zeros(1 << 20, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        kv.decode_attention_weights(t["q"], t["k"], t["v"], t["w"], t["tab"], t["ctx"],
+                                    workspace=host)
+    with pytest.raises(ValueError):
+        model.process_logits(t["x"], workspace=host)
+    with pytest.raises(ValueError):
+        model.process_logits(t["x"], out=t["x"][:, :4999].clone())
+
+
+def test_one_token_of_any_stride(dev):
+    """One token's rows may come from tensors of different token strides."""
+    say("one token")
+    t, freq, _ = small(dev)
+    wide = torch.zeros((1, HKV + 3, D), device=dev)
+    wide[:, :HKV] = t["vn"][:1]
+    pools = [[torch.zeros_like(t["k"]) for _ in "kv"] for _ in range(2)]
+    for v, p in ((t["vn"][:1], pools[0]), (wide[:, :HKV], pools[1])):
+        kv.rope_append(t["q"][:1], t["kn"][:1], v, t["pos"][:1], freq, *p, t["slots"][:1])
+    assert all(torch.equal(a, b) for a, b in zip(*pools)) and pools[0][1].any()
