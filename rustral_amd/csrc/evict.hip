@@ -19,8 +19,10 @@ constexpr int kBS = 16;
 // histogram in LDS of the keys that share the digits found so far, a sum over its
 // bins from the top, and the bin where it passes what is still wanted.  Counts are
 // integers, so their order does not matter.  It ends early where a bin is wanted
-// whole.  Keys are formed once and kept in LDS for up to kKeysMax positions (KEYS);
-// a longer context is read again by each of the passes.
+// whole.  The first digit is counted as the keys are formed; the keys of its bin are
+// then listed in LDS, if they are at most LIST, and the later digits are taken from the
+// list (else from all keys again).  Keys are kept in LDS for up to kKeysMax positions
+// (KEYS); a longer context is read again by each of the passes.
 // A wave owns a contiguous run of positions, so the kept ones' places need one
 // exchange of the waves' totals; inside a wave they come from ballots: with the
 // keys above the threshold and those that equal it counted apart, the place of a
@@ -28,10 +30,12 @@ constexpr int kBS = 16;
 // to the lower position.
 // Lane l of a step holds 4 positions, a float4 of one block.  The loops stay rolled:
 // a grid of few workgroups runs each instruction about once.
-// us for 8 layers x 16 sequences of U[1500, 4096] / 2 layers x 1 of 32,768, 8 KV
-// heads: 29.5 / 66 with keys in registers (unrolled) and 32 counts of the keys above
-// a candidate; 29.6 / 44.7 with keys in LDS and counts at candidates on a line
-// between the last two; 18.1 / 30.1 with the digits.
+// Bound by the round trips of its passes (loads 5 us, a pass over 32,768 keys in LDS
+// 2 to 4), far from its bytes.  us for 8 layers x 16 sequences of U[1500, 4096] / 2
+// layers x 1 of 32,768, 8 KV heads: 29.5 / 66 with keys in registers (unrolled) and 32
+// counts of the keys above a candidate; 29.6 / 44.7 with keys in LDS and counts at
+// candidates on a line between the last two; 17.1 / 26.1 with every digit taken from all
+// keys (23.8 / 42.8 without keys in LDS); 15.1 / 22.2 with the list.
 
 __device__ __forceinline__ uint32_t weight_key(float w) {
   const uint32_t u = __float_as_uint(w + 0.0f);  // -0 and +0 are one weight
@@ -65,11 +69,14 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
     int sinks, int recent, int cap) {
   constexpr int NW = NT / 64;
   constexpr int BPT = kBins / NT;  // bins a thread
+  constexpr int LIST = 4 * NT < 2048 ? 2048 : 4 * NT;
   extern __shared__ __align__(16) uint4 s_key[];  // KEYS: four positions each
   __shared__ __align__(16) uint32_t s_bin[kBins];
   __shared__ uint32_t s_sum[NW];
   __shared__ uint32_t s_found[3];  // the bin, its count, the count above it
-  __shared__ int2 s_tot[NW];
+  __shared__ uint32_t s_list[LIST];
+  __shared__ int s_above[NW], s_equal[NW];
+  __shared__ int s_listed;
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -104,48 +111,40 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
     if constexpr (KEYS) return g < groups ? s_key[g] : make_uint4(0u, 0u, 0u, 0u);
     else return form(g);
   };
-  if constexpr (KEYS) {
-#pragma unroll 4
-    for (int j = 0; j < steps; ++j) {
-      const int g = g0 + 64 * j;
-      const uint4 k = form(g);
-      if (g < groups) s_key[g] = k;
-    }
-  }
-
-  // Histogram of digit (key >> shift) % bins over the non-zero keys whose bits above
-  // are `top` (at shift + digit bits), and the bin from the top where the count
-  // reaches `want`: s_found.  Returns the histogram's total.
-  auto digit = [&](int shift, int bits, uint32_t top, uint32_t want) __attribute__((always_inline)) {
-    const uint32_t mask = (1u << bits) - 1u;
+  auto clear_bins = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < BPT; ++i) s_bin[tid + NT * i] = 0u;
     __syncthreads();
+  };
+  // Adds four keys' digits (key >> shift) % 2^bits to the bins: those of non-zero keys
+  // whose bits above are `top`.
+  auto add4 = [&](const uint4& k4, int shift, int bits, uint32_t top) __attribute__((always_inline)) {
+    const uint32_t mask = (1u << bits) - 1u;
     const int above = shift + bits;  // 32 for the first digit: no bits above
-#pragma unroll 2
-    for (int j = 0; j < steps; ++j) {
-      const uint4 k4 = keys(j);
-      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-      uint32_t d[4];
-      bool in[4];
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+    uint32_t d[4];
+    bool in[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        in[e] = k[e] != 0u && (above >= 32 || (k[e] >> (above & 31)) == top);
-        d[e] = (k[e] >> shift) & mask;
-      }
-      // one add for a wave whose 256 keys fall in one bin (equal sums, where every
-      // lane's add would wait for the others')
-      const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
-      const bool same = in[0] && in[1] && in[2] && in[3] && d[0] == d0 && d[1] == d0 &&
-                        d[2] == d0 && d[3] == d0;
-      if (__builtin_amdgcn_ballot_w64(!same) == 0) {
-        if (lane == 0) atomicAdd(&s_bin[d0], 256u);
-        continue;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (in[e]) atomicAdd(&s_bin[d[e]], 1u);
+    for (int e = 0; e < 4; ++e) {
+      in[e] = k[e] != 0u && (above >= 32 || (k[e] >> (above & 31)) == top);
+      d[e] = (k[e] >> shift) & mask;
     }
+    // one add for a wave whose 256 keys fall in one bin (equal sums, where every
+    // lane's add would wait for the others')
+    const uint32_t d0 = __builtin_amdgcn_readfirstlane(d[0]);
+    const bool same = in[0] && in[1] && in[2] && in[3] && d[0] == d0 && d[1] == d0 &&
+                      d[2] == d0 && d[3] == d0;
+    if (__builtin_amdgcn_ballot_w64(!same) == 0) {
+      if (lane == 0) atomicAdd(&s_bin[d0], 256u);
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (in[e]) atomicAdd(&s_bin[d[e]], 1u);
+  };
+  // The bin from the top where the bins' count reaches `want`: s_found.  Returns the
+  // bins' total.
+  auto find = [&](uint32_t want) __attribute__((always_inline)) {
     __syncthreads();
     // thread t has bins kBins - 1 - BPT t downwards: prefix sums from the top
     uint32_t c[BPT], mine = 0;
@@ -179,28 +178,100 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
     __syncthreads();
     return total;
   };
+  // A later digit over all keys.
+  auto digit_all = [&](int shift, int bits, uint32_t top, uint32_t want) __attribute__((always_inline)) {
+    clear_bins();
+#pragma unroll 2
+    for (int j = 0; j < steps; ++j) add4(keys(j), shift, bits, top);
+    find(want);
+  };
 
+  // The first digit, as the keys are formed.
+  if (tid == 0) s_listed = 0;
+  clear_bins();
+#pragma unroll 4
+  for (int j = 0; j < steps; ++j) {
+    const int g = g0 + 64 * j;
+    const uint4 k = form(g);
+    if constexpr (KEYS)
+      if (g < groups) s_key[g] = k;
+    add4(k, 21, 11, 0u);
+  }
+  const uint32_t present = find((uint32_t)budget);
   // thr and equal: a key is kept above thr, and `equal` of those that equal it
   uint32_t thr = 0u;
   int equal = 0;
-  const uint32_t present = digit(21, 11, 0u, (uint32_t)budget);
+  bool counted = false;  // s_above, s_equal hold the waves' totals
   const int n = present < (uint32_t)budget ? (int)present : budget;
   if (present > (uint32_t)n) {
-    uint32_t top = s_found[0], want = (uint32_t)n - s_found[2];
+    const uint32_t t1 = s_found[0], held = s_found[1];
+    uint32_t top = t1, want = (uint32_t)n - s_found[2];
     int shift = 21;
-    bool whole = s_found[1] == want;
-    if (!whole) {
-      digit(10, 11, top, want);
+    bool whole = held == want;
+    if (!whole && held <= (uint32_t)LIST) {
+      // list the bin's keys (their low 21 bits, the wave above) and count those above
+      // the bin, then go on with the list
+      int na = 0;
+#pragma unroll 4
+      for (int j = 0; j < steps; ++j) {
+        const uint4 k4 = keys(j);
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+        uint64_t in[4];
+        int count = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          na += __popcll(__builtin_amdgcn_ballot_w64((k[e] >> 21) > t1));
+          in[e] = __builtin_amdgcn_ballot_w64((k[e] >> 21) == t1 && k[e] != 0u);
+          count += __popcll(in[e]);
+        }
+        if (count == 0) continue;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&s_listed, count);
+        at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int mine = __builtin_amdgcn_mbcnt_hi(
+              (uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], at));
+          if ((in[e] >> lane) & 1u) s_list[mine] = (k[e] & 0x1fffffu) | (uint32_t)w << 21;
+          at += __popcll(in[e]);
+        }
+      }
+      if (lane == 0) s_above[w] = na, s_equal[w] = 0;
+      auto digit_list = [&](int shift_, int bits, uint32_t low) __attribute__((always_inline)) {
+        clear_bins();
+        for (uint32_t i = tid; i < held; i += NT) {
+          const uint32_t k = s_list[i] & 0x1fffffu;
+          if (bits == 11 || k >> 10 == low) atomicAdd(&s_bin[(k >> shift_) & ((1u << bits) - 1u)], 1u);
+        }
+        find(want);
+      };
+      digit_list(10, 11, 0u);
+      top = t1 << 11 | s_found[0], want -= s_found[2], shift = 10;
+      whole = s_found[1] == want;
+      if (!whole) {
+        digit_list(0, 10, s_found[0]);
+        top = top << 10 | s_found[0], want -= s_found[2], shift = 0;
+      }
+      counted = true;
+    } else if (!whole) {
+      digit_all(10, 11, top, want);
       top = top << 11 | s_found[0], want -= s_found[2], shift = 10;
       whole = s_found[1] == want;
       if (!whole) {
-        digit(0, 10, top, want);
+        digit_all(0, 10, top, want);
         top = top << 10 | s_found[0], want -= s_found[2], shift = 0;
       }
     }
     // a whole bin: everything from its first key on
     if (whole) thr = top ? (top << shift) - 1u : 0u;
     else thr = top, equal = (int)want;
+    if (counted) {
+      for (uint32_t i = tid; i < held; i += NT) {
+        const uint32_t e = s_list[i], k = t1 << 21 | (e & 0x1fffffu);
+        if (k > thr) atomicAdd(&s_above[e >> 21], 1);
+        else if (k == thr) atomicAdd(&s_equal[e >> 21], 1);
+      }
+    }
   }
   if (h == 0 && layer == 0 && tid == 0) new_lens[b] = n;
 
@@ -210,25 +281,25 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
       keep + (((int64_t)layer * gridDim.y + b) * num_kv_heads + h) * budget;
   auto place = [&](auto with) __attribute__((always_inline)) {
     constexpr bool EQ = decltype(with)::value;
-    int na = 0, ne = 0;
+    if (!counted) {
+      int na = 0, ne = 0;
 #pragma unroll 4
-    for (int j = 0; j < steps; ++j) {
-      const uint4 k4 = keys(j);
-      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+      for (int j = 0; j < steps; ++j) {
+        const uint4 k4 = keys(j);
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        na += __popcll(__builtin_amdgcn_ballot_w64(k[e] > thr));
-        if constexpr (EQ) ne += __popcll(__builtin_amdgcn_ballot_w64(k[e] == thr));
+        for (int e = 0; e < 4; ++e) {
+          na += __popcll(__builtin_amdgcn_ballot_w64(k[e] > thr));
+          if constexpr (EQ) ne += __popcll(__builtin_amdgcn_ballot_w64(k[e] == thr));
+        }
       }
+      if (lane == 0) s_above[w] = na, s_equal[w] = ne;
     }
-    if (lane == 0) s_tot[w] = make_int2(na, ne);
     __syncthreads();
     int xa = 0, xe = 0;
 #pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      const int2 v = s_tot[x];
-      if (x < w) xa += v.x, xe += v.y;
-    }
+    for (int x = 0; x < NW; ++x)
+      if (x < w) xa += s_above[x], xe += s_equal[x];
 #pragma unroll 2
     for (int j = 0; j < steps; ++j) {
       const uint4 k4 = keys(j);
@@ -439,8 +510,16 @@ extern "C" int rkv_evict_select(int32_t* keep, int32_t* new_lens, const float* w
   evict_select_kernel<NT, K><<<grid, NT, K ? (size_t)(cap + 3) / 4 * 16 : 0, s>>>(             \
       keep, new_lens, weights, weights_layer_stride, block_tables, max_blocks_per_seq, ctx_lens, \
       num_kv_heads, num_blocks, budget, sinks, recent, cap)
-  // 256 threads up to 4,096 positions, so that several workgroups share a CU
-  if (cap <= 4096) RKV_SELECT(256, true);
+  // Threads: where the workgroups leave CUs idle each runs wide, where several share a
+  // CU fewer threads wait for each other's barriers.  us with 256 / 512 / 1,024 threads:
+  //   128 workgroups, 700 positions 5.1 / 5.0 / 6.0; 2,000 7.2 / 6.0 / 7.3; 4,000 9.8 /
+  //   7.6 / 7.8; 8,000 16.5 / 10.8 / 10.0; 32,000 61 / 35 / 26
+  //   1,024 workgroups, 2,000 9.2 / 10.7 / 21.8; 4,000 15.0 / 16.6 / 26.0; 8,000 36.6 /
+  //   26.8 / 35.9; 16,000 68 / 48 / 58; 32,000 232 / 133 / 99
+  const bool crowded = (int64_t)num_kv_heads * num_seqs * n_layers > 512;
+  const int narrow = crowded ? 4096 : 1024;
+  if (cap <= narrow) RKV_SELECT(256, true);
+  else if (cap <= 4 * narrow) RKV_SELECT(512, true);
   else if (cap <= kKeysMax) RKV_SELECT(1024, true);
   else RKV_SELECT(1024, false);
 #undef RKV_SELECT

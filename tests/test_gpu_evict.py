@@ -229,3 +229,38 @@ def test_evict_front_end_refuses(dev):
         kv.evict_compact(k, k, keep[:, :1], ctx, tab, tab)
     with pytest.raises(ValueError):
         kv.evict_compact(k, k, keep, ctx, tab, tab, weights=w[:2])
+
+
+def _sums(rng, kind, shape):
+    x = rng.standard_normal(shape)
+    w = {"spread": lambda: np.exp(2 * x),              # a few hundred keys a first digit
+         "close": lambda: 1 + 1e-4 * x,                # nearly all keys in one first digit
+         "steps": lambda: np.round(np.exp(x) * 4) / 4,  # ties at every threshold
+         "nan": lambda: np.where(x > -0.5, np.nan, x),  # the threshold among the NaN
+         "tiny": lambda: x * 1e-42}[kind]()            # subnormal sums, both signs
+    return w.astype(np.float32)
+
+
+@pytest.mark.parametrize("kind", ["spread", "close", "steps", "nan", "tiny"])
+@pytest.mark.parametrize("length,B,layers", [(1, 2, 1), (300, 2, 1), (1500, 3, 1), (6000, 1, 2),
+                                             (33000, 1, 1), (150, 80, 4), (2500, 2, 150)])
+def test_select_distributions(dev, kind, length, B, layers):
+    """Where the threshold falls decides how the kernel comes to it: in a first digit of
+    few keys or of many, among ties, among the lowest keys; for few workgroups and for
+    many, with budgets of one row, a part and all but one."""
+    say(f"select {kind} {length} x {B} x {layers}")
+    rng = np.random.default_rng(length + B)
+    hkv = 2
+    ctx = contexts(rng, B, max(1, length - 40), length)
+    nb = int(((ctx + 15) // 16).sum()) + 1
+    tables = make_tables(rng, ctx, 16, nb)
+    one = _sums(rng, kind, (2, nb, hkv, 16))
+    w = one[np.arange(layers) % 2]
+    for budget in sorted({1, int(ctx.max()) // 3 + 1, max(1, int(ctx.min()) - 1)}):
+        keep, lens = kv.evict_select(to_dev(w, dev), to_dev(tables, dev), to_dev(ctx, dev), budget,
+                                     sinks=min(2, budget - 1), recent=0)
+        for i in range(min(2, layers)):
+            want, want_lens = R.select(one[i], tables, ctx, budget, min(2, budget - 1), 0)
+            assert np.array_equal(to_np(lens), want_lens)
+            got = to_np(keep)[i::2]
+            assert all(np.array_equal(g, want) for g in got), (budget, i)
