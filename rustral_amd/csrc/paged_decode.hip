@@ -245,8 +245,13 @@ __global__ __launch_bounds__(256) void decode_merge_rows_kernel(
 // costs the partition pass 19 us (104 to 123): all workgroups writing one place
 // cost nothing, a quarter of the bytes 6 us, half 13, so it is where the rows land
 // in memory, not the stores; streaming and write-through hints made it no faster.
-constexpr int kWeightTokens = 1024;
-constexpr int kWaveMergeParts = 16;  // up to so many partitions a wave merges a head
+// us with 256 / 512 / 1,024 / 2,048 positions a workgroup: 137.3 / 135.4 / 135.9 /
+// 136.1; one sequence of 2,000: 11.4 / 11.7 / 12.3 / 13.1; 8 x U[16384, 65536]: 279 /
+// 276 / 276 / 277.
+constexpr int kWeightTokens = 512;
+// Up to so many partitions a wave merges a head: 64 x U[512, 4096] (8 partitions) 135.9
+// where a workgroup a head takes 140.9; 2 x U[30000, 60000] (94) 79.9 against 77.0.
+constexpr int kWaveMergeParts = 16;
 
 template <int G, int D>
 __global__ __launch_bounds__(256) void decode_merge_weights_kernel(

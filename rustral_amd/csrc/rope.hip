@@ -11,6 +11,11 @@
 // fraction before it is rounded to 32: in 32 bits the product alone is off by
 // p f 2^-24 rad, 0.06 rad at a million positions.  A float fraction of a turn
 // in [-1/2, 1/2] is off by 2^-26 turns at most, 1e-7 rad.
+//
+// Every element is read and written once, a lane's in 16-byte pieces.  Bound by HBM for
+// a prompt: 8,192 tokens of 32 query and 8 KV heads of 128 into a bf16 pool 69 us (368
+// MB, 5.3 TB/s; a copy reaches 5.1), 16,384 x 16 half-rotated heads of 64 alone 27 us (4.9 TB/s);
+// by its launch for a decode step: 64 tokens 3.9 us.
 #include "common.hpp"
 
 #include <cmath>
@@ -287,7 +292,9 @@ Layout layout_of(int interleaved, int rotary_dim) {
 // Threads of a workgroup (whole rows) and workgroups a token's rows are split
 // over: one row a thread while that leaves fewer workgroups than kFill, so that
 // a decode step's few tokens spread over the chip; then every row of a token in
-// one workgroup, which takes the sines once.
+// one workgroup, which takes the sines once.  us for 64 tokens of 32 + 2 x 8 rows of 128:
+// split 3.9, one workgroup a token 4.3; for 8,192 tokens: split three ways 70.3, one
+// workgroup 69.1.
 constexpr int64_t kFill = 2048;
 void shape_of(int64_t n_tokens, int rows, int lpr, unsigned& threads, unsigned& splits) {
   const int most = 256 / lpr;
