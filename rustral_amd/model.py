@@ -406,19 +406,19 @@ def process_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
         return t.data_ptr()
 
     if out is None:
-        out = torch.empty((rows, n), dtype=f32, device=logits.device)
+        out = logits.new_empty((rows, n))
     ostride = out.stride()
     if out.dtype is not f32 or out.shape != (rows, n) or out.get_device() != dev or \
             (ostride[1] != 1 and n > 1):
         raise ValueError("out must be fp32 of the logits' shape with contiguous rows, on their device")
     if pick is None:
-        pick = torch.empty(rows, dtype=i32, device=logits.device)
+        pick = logits.new_empty(rows, dtype=i32)
     ws_bytes, ws = _logits_workspace(rows, n), None
     if workspace is not None:
         _one_device(dev, ((_dev(workspace, "workspace"), "workspace"),))
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif ws_bytes:
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
+        workspace = logits.new_empty(ws_bytes, dtype=torch.uint8)
         ws = workspace.data_ptr()
     words = 0
     if allowed is not None:
