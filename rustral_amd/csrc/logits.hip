@@ -9,8 +9,8 @@
 // a pick needs.  Bound by the read and write of the logits for large batches,
 // by the two launches for single rows.  us for 1 x 32,000 / 64 x 128,256 columns
 // (histories of 300 / 2,048 at most) by columns and threads a workgroup: 4,096 with
-// 256 threads 9.7 / 27.0, with 512 7.7 / 23.2; 2,048 with 128 9.6 / 28.0, with 256
-// 7.5 / 23.3; 8,192 with 512 10.1 / 27.3, with 1,024 8.2 / 23.7.
+// 512 7.6 / 22.3 (with the mask and the history requested only after the first barrier
+// 7.8 / 22.8); 2,048 with 256 7.4 / 23.2; 8,192 with 1,024 8.4 / 23.1.
 #include "../../include/rustral_model.h"
 #include "common.hpp"
 
@@ -85,26 +85,45 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(LogitsArgs p) 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[i][e] = c + e < cols ? x[c + e] : 0.0f;
   }
+  // Everything that does not wait for the LDS counters is requested before the first
+  // barrier: the mask's words and the first of the history and of the biases.
+  const uint32_t* mask = p.allowed ? reinterpret_cast<const uint32_t*>(p.allowed) +
+                                         (int64_t)r * p.allowed_stride
+                                   : nullptr;
+  uint32_t bits[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    // c0 and c are multiples of VEC: one word of the mask holds all VEC bits
+    const int c = VEC * (tid + kThreads * i);
+    bits[i] = mask && c < cols ? mask[(c0 + c) >> 5] >> ((c0 + c) & 31) : 0xffffffffu;
+  }
   const bool counts = p.repetition || p.frequency || p.presence;
   const int h0 = counts ? p.history_start[r] : 0, h1 = counts ? p.history_start[r + 1] : 0;
   const int made = h0 + (counts && p.prompt_lens ? p.prompt_lens[r] : 0);
   const int b0 = p.bias_ids ? p.bias_start[r] : 0, b1 = p.bias_ids ? p.bias_start[r + 1] : 0;
+  const float rep = p.repetition ? p.repetition[r] : 1.0f;
+  const float freq = p.frequency ? p.frequency[r] : 0.0f;
+  const float pres = p.presence ? p.presence[r] : 0.0f;
   const bool use_h = h1 > h0, use_b = b1 > b0;  // workgroup-uniform
   if (use_h || use_b) {
-    for (int i = tid; i < kSlice / 4; i += kThreads) {
-      if (use_h) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (use_b) reinterpret_cast<uint4*>(s_bias)[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    __syncthreads();
     // kAhead ids a thread requested together: a row's history is read by every
     // slice, and one id at a time each wait is a round trip
-    for (int at = h0; at < h1; at += kAhead * kThreads) {
-      int id[kAhead];
+    int id[kAhead];
+    auto ids = [&](int at) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int i = at + tid + kThreads * u;
         id[u] = i < h1 ? p.history[i] : -1;
       }
+    };
+    ids(h0);
+    int bias_id = b0 + tid < b1 ? p.bias_ids[b0 + tid] : -1;
+    for (int i = tid; i < kSlice / 4; i += kThreads) {
+      if (use_h) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (use_b) reinterpret_cast<uint4*>(s_bias)[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __syncthreads();
+    for (int at = h0; at < h1; at += kAhead * kThreads) {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         if (id[u] >= c0 && id[u] - c0 < cols) {
@@ -112,27 +131,21 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(LogitsArgs p) 
           else atomicAdd(&s_count[id[u] - c0], 1u);
         }
       }
+      if (at + kAhead * kThreads < h1) ids(at + kAhead * kThreads);
     }
     for (int i = b0 + tid; i < b1; i += kThreads) {
-      const int id = p.bias_ids[i];
-      if (id >= c0 && id - c0 < cols) atomicMax(&s_bias[id - c0], (uint32_t)(i - b0) + 1u);
+      if (bias_id >= c0 && bias_id - c0 < cols)
+        atomicMax(&s_bias[bias_id - c0], (uint32_t)(i - b0) + 1u);
+      bias_id = i + kThreads < b1 ? p.bias_ids[i + kThreads] : -1;
     }
     __syncthreads();
   }
-  const float rep = p.repetition ? p.repetition[r] : 1.0f;
-  const float freq = p.frequency ? p.frequency[r] : 0.0f;
-  const float pres = p.presence ? p.presence[r] : 0.0f;
-  const uint32_t* mask = p.allowed ? reinterpret_cast<const uint32_t*>(p.allowed) +
-                                         (int64_t)r * p.allowed_stride
-                                   : nullptr;
   float* out = p.out ? p.out + (int64_t)r * p.out_stride + c0 : nullptr;
   Best best{-INFINITY, -1};
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
     const int c = VEC * (tid + kThreads * i);
     if (c >= cols) continue;
-    // c0 and c are multiples of VEC: one word of the mask holds all VEC bits
-    const uint32_t bits = mask ? mask[(c0 + c) >> 5] >> ((c0 + c) & 31) : 0xffffffffu;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       if (c + e >= cols) continue;
@@ -149,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(LogitsArgs p) 
         const uint32_t at = s_bias[c + e];
         if (at) y += p.bias[b0 + (int)at - 1];
       }
-      y = (bits >> e) & 1u ? y : -INFINITY;
+      y = (bits[i] >> e) & 1u ? y : -INFINITY;
       v[i][e] = y;
       if (y > -INFINITY) best = better(best, Best{y, c0 + c + e});  // a NaN is not
     }
