@@ -359,23 +359,26 @@ __global__ __launch_bounds__(256) void evict_compact_kernel(
   const int64_t unit = (int64_t)blockIdx.x * 4 + w;
   const int j = (int)(unit / num_kv_heads), h = (int)(unit - (int64_t)j * num_kv_heads);
   const int b = blockIdx.y, layer = blockIdx.z;
+  if (j >= dst_blocks) return;
+  // One round trip for what the arguments alone place (keep past new_lens is within its
+  // row of the array), then the source table, then the rows.
+  const int row = lane & 15;
+  const int at = j * kBS + row;
+  int32_t p = at < budget
+                  ? keep[(((int64_t)layer * gridDim.y + b) * num_kv_heads + h) * budget + at]
+                  : -1;
+  const int32_t dst = dst_tables[(int64_t)b * dst_blocks + j];
   int n = new_lens[b];
   n = n > budget ? budget : n;
-  if (j >= dst_blocks || (int64_t)j * kBS >= n) return;
-  const int32_t dst = dst_tables[(int64_t)b * dst_blocks + j];
-  if (dst < 0 || dst >= num_blocks) return;
+  if (at >= n) p = -1;
+  if ((int64_t)j * kBS >= n || dst < 0 || dst >= num_blocks) return;
   // source row (in rows of the layer's pool) of destination row lane, or -1
-  const int row = lane & 15;
   int64_t from = -1;
   int32_t sblk = -1;
-  if (j * kBS + row < n) {
-    const int32_t p = keep[(((int64_t)layer * gridDim.y + b) * num_kv_heads + h) * budget +
-                           j * kBS + row];
-    if (p >= 0 && p < src_blocks * kBS) {
-      sblk = src_tables[(int64_t)b * src_blocks + p / kBS];
-      if (sblk >= 0 && sblk < num_blocks)
-        from = ((int64_t)sblk * num_kv_heads + h) * kBS + p % kBS;
-    }
+  if (p >= 0 && p < src_blocks * kBS) {
+    sblk = src_tables[(int64_t)b * src_blocks + p / kBS];
+    if (sblk >= 0 && sblk < num_blocks)
+      from = ((int64_t)sblk * num_kv_heads + h) * kBS + p % kBS;
   }
   const bool live = from >= 0;
   const int64_t to = ((int64_t)dst * num_kv_heads + h) * kBS;

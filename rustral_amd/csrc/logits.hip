@@ -10,7 +10,8 @@
 // by the two launches for single rows.  us for 1 x 32,000 / 64 x 128,256 columns
 // (histories of 300 / 2,048 at most) by columns and threads a workgroup: 4,096 with
 // 512 7.6 / 22.3 (with the mask and the history requested only after the first barrier
-// 7.8 / 22.8); 2,048 with 256 7.4 / 23.2; 8,192 with 1,024 8.4 / 23.1.
+// 7.8 / 22.8); 2,048 with 256 7.4 / 23.2; 8,192 with 1,024 8.4 / 23.1.  With streaming
+// stores 7.7 / 21.3; streaming loads as well 22.9 (a caller's logits are often cached).
 #include "../../include/rustral_model.h"
 #include "common.hpp"
 
@@ -169,7 +170,8 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(LogitsArgs p) 
     if (out) {
       if constexpr (VEC == 4) {
         if (c + 3 < cols) {
-          *reinterpret_cast<float4*>(out + c) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+          store_stream(out + c, __builtin_bit_cast(uint4, make_float4(v[i][0], v[i][1], v[i][2],
+                                                                      v[i][3])));
           continue;
         }
       }
