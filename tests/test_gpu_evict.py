@@ -264,3 +264,62 @@ def test_select_distributions(dev, kind, length, B, layers):
             assert np.array_equal(to_np(lens), want_lens)
             got = to_np(keep)[i::2]
             assert all(np.array_equal(g, want) for g in got), (budget, i)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (4, 4, 64), (16, 2, 64), (4, 2, 128)])
+def test_what_no_table_names_is_not_seen(dev, kind, hq, hkv, d):
+    """Block 0 (what an invalid id is read as), a block past every table and the rows behind
+    each context hold NaN and infinities, scales too; tables have holes, ids too large,
+    a context past its table's valid part and one of length 0."""
+    say(f"unseen {kind} hq={hq} hkv={hkv} d={d}")
+    rng = np.random.default_rng(21)
+    ctx = np.array([37, 0, 700, 130, 16], np.int32)
+    nb = 60
+    ids = rng.permutation(np.arange(1, nb - 1))
+    tables = np.full((5, 45), -1, np.int32)
+    o = 0
+    for b, n in enumerate(ctx):
+        m = -(-int(n) // 16)
+        if b == 2:
+            m = 30                              # the rest of its context has no blocks
+        tables[b, :m] = ids[o:o + m]
+        o += m
+    tables[2, 3], tables[3, 0], tables[3, 4] = -1, nb, 2 ** 31 - 1
+    (k, v, ks, vs), (fk, fv) = pools_of(rng, nb, hkv, d, kind)
+    bad = {"f32": np.float32("nan"), "bf16": np.uint16(0x7fc0)}.get(kind, np.uint8(0x7f))
+    inf = {"f32": np.float32("inf"), "bf16": np.uint16(0xff80)}.get(kind, np.uint8(0xff))
+    for blk in (0, nb - 1):
+        k[blk], v[blk] = bad, inf
+        if ks is not None:
+            ks[blk], vs[blk] = np.nan, np.inf
+    for b, n in enumerate(ctx):
+        if n % 16 and 0 <= tables[b, n // 16] < nb:
+            k[tables[b, n // 16], :, n % 16:] = bad
+            v[tables[b, n // 16], :, n % 16:] = inf
+            if kind in ("int8", "fp8"):
+                ks[tables[b, n // 16], :, n % 16:] = np.nan
+                vs[tables[b, n // 16], :, n % 16:] = np.inf
+    fk, fv = np.nan_to_num(fk), np.nan_to_num(fv)
+    q = rng.standard_normal((5, hq, d)).astype(np.float32)
+    fmt = kind if kind not in ("f32", "bf16") else None
+    scales = dict(k_scale=to_dev(ks, dev), v_scale=to_dev(vs, dev)) if fmt else {}
+    want, bound, ws, _ = R.attend(q, fk, fv, tables, ctx, 1 / math.sqrt(d))
+    w = torch.zeros((nb, hkv, 16), device=dev)
+    gk, gv, gt, gc = (to_dev(a, dev) for a in (k, v, tables, ctx))
+    out = kv.decode_attention_weights(to_dev(q, dev), gk, gv, w, gt, gc, fmt=fmt, **scales)
+    R.assert_within(to_np(out), want, bound, "attention with weights")
+    w = to_np(w)
+    assert np.isfinite(w).all() and not w[0].any() and not w[nb - 1].any()
+    assert abs(w.sum() - 4 * hq) < 1e-2
+    if kind.endswith("block"):
+        args = (gk, gv, scales["k_scale"], scales["v_scale"], gt)
+        for ps in (0, 64, 128):
+            got = kv.decode_attention_q(to_dev(q, dev), *args, gc, None, fmt, partition_size=ps)
+            R.assert_within(to_np(got), want, bound, f"decode {ps}")
+        n = np.array([37, 0, 90, 100, 16], np.int32)
+        start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+        qq = rng.standard_normal((int(start[-1]), hq, d)).astype(np.float32)
+        got = kv.prefill_attention_q(to_dev(qq, dev), *args, to_dev(start, dev), gc, None, fmt)
+        want, bound, _, _ = R.attend(qq, fk, fv, tables, ctx, 1 / math.sqrt(d), n, start)
+        R.assert_within(to_np(got), want, bound, "prefill")

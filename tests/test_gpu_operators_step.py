@@ -373,3 +373,62 @@ def test_one_token_of_any_stride(dev):
     for v, p in ((t["vn"][:1], pools[0]), (wide[:, :HKV], pools[1])):
         kv.rope_append(t["q"][:1], t["kn"][:1], v, t["pos"][:1], freq, *p, t["slots"][:1])
     assert all(torch.equal(a, b) for a, b in zip(*pools)) and pools[0][1].any()
+
+
+@pytest.mark.parametrize("fmt", [None, "int8_block", "fp8_block"])
+def test_pools_past_32_bit_offsets(dev, fmt):
+    """Two layers of 70,000 blocks of 8 x 128 (2.3e9 elements), the blocks in use at their
+    ends: the same bits as in pools that hold only those."""
+    say(f"large pools fmt={fmt}")
+    hkv, d, hq, big = 8, 128, 16, 70_000
+    ids = np.array([big - 1, 3, big - 2, 65_600, big - 5, 1, big - 9, 40_001, big - 7], np.int64)
+    few = len(ids)
+    ctx = np.array([33, 20], np.int32)
+    tab = np.array([[0, 1, 2], [3, 4, -1]], np.int32)      # places in ids
+    dst = np.array([[5, 6], [7, 8]], np.int32)
+    rng = np.random.default_rng(2)
+    total = int(ctx.sum())
+    kn, vn = (to_dev(rng.standard_normal((2, total, hkv, d)).astype(np.float32), dev) for _ in "kv")
+    q = to_dev(rng.standard_normal((2, hq, d)).astype(np.float32), dev)
+    qq = to_dev(rng.standard_normal((total, hq, d)).astype(np.float32), dev)
+    start = to_dev(np.array([0, 33, 53], np.int32), dev)
+    gctx = to_dev(ctx, dev)
+    freq, _ = kv.rope_frequencies(d, device=dev)
+    pos = to_dev(np.concatenate([np.arange(n) for n in ctx]).astype(np.int32), dev)
+    results = []
+    for nb in (few, big):
+        name = np.arange(few) if nb == few else ids
+        to = lambda t: to_dev(np.where(t >= 0, name[t], -1).astype(np.int32), dev)
+        dt = torch.bfloat16 if fmt is None else torch.uint8
+        k, v = (torch.zeros((2, nb, hkv, 16, d), dtype=dt, device=dev) for _ in "kv")
+        w = torch.zeros((2, nb, hkv, 16), device=dev)
+        ks, vs = (torch.zeros((2, nb, hkv), device=dev) for _ in "kv")
+        gt, gd = to(tab), to(dst)
+        out = []
+        if fmt is None:
+            slots = np.concatenate([name[tab[b, np.arange(n) // 16]] * 16 + np.arange(n) % 16
+                                    for b, n in enumerate(ctx)])
+            for i in range(2):
+                out.append(kv.rope_append(qq, kn[i], vn[i], pos, freq, k[i], v[i],
+                                          to_dev(slots.astype(np.int64), dev)))
+            sc = [{}] * 2
+        else:
+            kv.append_block_q(k, v, ks, vs, kn, vn, start, gt, gctx, fmt)
+            sc = [dict(k_scale=ks[i], v_scale=vs[i], fmt=fmt) for i in range(2)]
+        for i in range(2):
+            out.append(kv.decode_attention_weights(q, k[i], v[i], w[i], gt, gctx, **sc[i]))
+            if fmt:
+                out.append(kv.decode_attention_q(q, k[i], v[i], ks[i], vs[i], gt, gctx, fmt=fmt))
+                out.append(kv.prefill_attention_q(qq, k[i], v[i], ks[i], vs[i], gt, start, gctx,
+                                                  fmt=fmt))
+                out += kv.gather_q(k[i], v[i], ks[i], vs[i], gt, gctx, fmt=fmt)
+        keep, left = kv.evict_select(w, gt, gctx, 18, sinks=2, recent=3)
+        kv.evict_compact(k, v, keep, left, gt, gd, weights=w,
+                         **(dict(k_scale=ks, v_scale=vs, fmt=fmt) if fmt else {}))
+        at = torch.from_numpy(name).to(dev)
+        out += [keep, left] + [t[:, at].contiguous() for t in (k, v, w, ks, vs)]
+        results.append(out)
+        del k, v
+    assert results[0][-5].any() and results[0][-3].any()
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
