@@ -337,6 +337,8 @@ def _bcode(fmt) -> int:
 def _scale_shapes(k_shape, v_shape, ks_shape, vs_shape, code: int) -> None:
     """Scale pools of the shape their format has: one a row, or one a tile.  The
     kernels index them by the byte pools' shape."""
+    if v_shape != k_shape:
+        raise ValueError("k_pool and v_pool must have one shape")
     cut = -2 if code >= _lib.RKV_I8_BLOCK else -1
     if ks_shape != k_shape[:cut] or vs_shape != v_shape[:cut]:
         raise ValueError("scale pools must be the byte pools' shape without head_dim, and for the "
@@ -620,13 +622,25 @@ def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
     """prefill_attention over block-scaled 8-bit pools ('int8_block',
     'fp8_block')."""
     code = _bcode(fmt)
-    _dev(q, "q", torch.float32), _dev(k_pool, "k_pool", torch.uint8)
-    _dev(v_pool, "v_pool", torch.uint8), _dev(q_start, "q_start", torch.int32)
-    _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
-    _scale_pools(k_pool, v_pool, k_scale, v_scale, code)
-    _one_device(q.get_device(), ((k_pool, "k_pool"), (v_pool, "v_pool"), (k_scale, "k_scale"),
-                                 (v_scale, "v_scale"), (q_start, "q_start"),
-                                 (block_tables, "block_tables"), (ctx_lens, "ctx_lens")))
+    u8, f32, i32 = torch.uint8, torch.float32, torch.int32
+    dev = q.get_device()
+    if not (q.dtype is f32 and k_pool.dtype is u8 and v_pool.dtype is u8 and
+            k_scale.dtype is f32 and v_scale.dtype is f32 and block_tables.dtype is i32 and
+            q_start.dtype is i32 and ctx_lens.dtype is i32 and q.is_contiguous() and
+            k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and
+            v_scale.is_contiguous() and block_tables.is_contiguous() and
+            q_start.is_contiguous() and ctx_lens.is_contiguous() and dev >= 0 and
+            dev == k_pool.get_device() == v_pool.get_device() == k_scale.get_device() ==
+            v_scale.get_device() == block_tables.get_device() == q_start.get_device() ==
+            ctx_lens.get_device()):
+        _dev(q, "q", f32), _dev(k_pool, "k_pool", u8)  # says which and why
+        _dev(v_pool, "v_pool", u8), _dev(k_scale, "k_scale", f32)
+        _dev(v_scale, "v_scale", f32), _dev(q_start, "q_start", i32)
+        _dev(block_tables, "block_tables", i32), _dev(ctx_lens, "ctx_lens", i32)
+        _one_device(dev, ((k_pool, "k_pool"), (v_pool, "v_pool"), (k_scale, "k_scale"),
+                          (v_scale, "v_scale"), (q_start, "q_start"),
+                          (block_tables, "block_tables"), (ctx_lens, "ctx_lens")))
+    _scale_shapes(k_pool.shape, v_pool.shape, k_scale.shape, v_scale.shape, code)
     check_attention_shapes(q.shape, k_pool.shape, block_tables.shape, ctx_lens.shape,
                            q_start.shape)
     nb, hkv, bs, d = k_pool.shape
@@ -639,7 +653,7 @@ def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         out = torch.zeros_like(q)
     else:
         _out_like(out, q)
-    _launch(q.get_device(), lib().rkv_prefill_attention_q, out.data_ptr(), q.data_ptr(),
+    _launch(dev, lib().rkv_prefill_attention_q, out.data_ptr(), q.data_ptr(),
             k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
             block_tables.data_ptr(), block_tables.shape[1], q_start.data_ptr(),
             ctx_lens.data_ptr(), B, q.shape[1], hkv, d, bs, nb, max_q_len, float(scale), code)
@@ -812,19 +826,29 @@ def decode_attention_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
     the softmax weight each cached row received, summed over its KV head's query
     heads.  fmt None: fp32 or bf16 pools; else a 1-byte format with its scale
     pools.  workspace: weights_workspace_bytes."""
-    _dev(q, "q", torch.float32), _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool")
-    _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
-    _dev(weights, "weights", torch.float32)
-    check_attention_shapes(q.shape, k_pool.shape, block_tables.shape, ctx_lens.shape)
-    if weights.shape != k_pool.shape[:3]:
+    f32, i32 = torch.float32, torch.int32
+    dev = q.get_device()
+    if not (q.dtype is f32 and weights.dtype is f32 and block_tables.dtype is i32 and
+            ctx_lens.dtype is i32 and q.is_contiguous() and weights.is_contiguous() and
+            k_pool.is_contiguous() and v_pool.is_contiguous() and
+            block_tables.is_contiguous() and ctx_lens.is_contiguous() and dev >= 0 and
+            dev == k_pool.get_device() == v_pool.get_device() == weights.get_device() ==
+            block_tables.get_device() == ctx_lens.get_device()):
+        _dev(q, "q", f32), _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool")  # says which and why
+        _dev(block_tables, "block_tables", i32), _dev(ctx_lens, "ctx_lens", i32)
+        _dev(weights, "weights", f32)
+        _one_device(dev, ((k_pool, "k_pool"), (v_pool, "v_pool"), (weights, "weights"),
+                          (block_tables, "block_tables"), (ctx_lens, "ctx_lens")))
+    shape, tables = k_pool.shape, block_tables.shape
+    check_attention_shapes(q.shape, shape, tables, ctx_lens.shape)
+    if weights.shape != shape[:3]:
         raise ValueError("weights must be the pools' shape without head_dim")
     code, ks, vs = _pool_code(k_pool, v_pool, k_scale, v_scale, fmt)
-    _one_device(q.get_device(), ((k_pool, "k_pool"), (v_pool, "v_pool"), (weights, "weights"),
-                                 (block_tables, "block_tables"), (ctx_lens, "ctx_lens"),
-                                 (k_scale, "k_scale"), (v_scale, "v_scale")))
-    nb, hkv, bs, d = k_pool.shape
+    if ks is not None:
+        _one_device(dev, ((k_scale, "k_scale"), (v_scale, "v_scale")))
+    nb, hkv, bs, d = shape
     B, hq, _ = q.shape
-    mbs = block_tables.shape[1]
+    mbs = tables[1]
     if max_context is None:
         max_context = mbs * bs
     if scale is None:
@@ -837,8 +861,8 @@ def decode_attention_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
         need = weights_workspace_bytes(B, hq, hkv, d, max_context)
         workspace = q.new_empty(max(need, 16), dtype=torch.uint8)
     else:
-        _one_device(q.get_device(), ((_dev(workspace, "workspace"), "workspace"),))
-    _launch(q.get_device(), lib().rkv_decode_attention_weights, out.data_ptr(), weights.data_ptr(),
+        _one_device(dev, ((_dev(workspace, "workspace"), "workspace"),))
+    _launch(dev, lib().rkv_decode_attention_weights, out.data_ptr(), weights.data_ptr(),
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks, vs, block_tables.data_ptr(),
             mbs, ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, max_context, float(scale), code,
             workspace.data_ptr(), workspace.numel() * workspace.element_size())
@@ -853,13 +877,19 @@ def evict_select(weights: torch.Tensor, block_tables: torch.Tensor, ctx_lens: to
     position), `budget` in all.  weights [num_blocks, Hkv, 16] or [n_layers, ..].
     Returns (keep int32 [.., B, Hkv, budget], ascending, -1 behind the last;
     new_lens int32 [B])."""
-    _dev(weights, "weights", torch.float32)
-    _dev(block_tables, "block_tables", torch.int32), _dev(ctx_lens, "ctx_lens", torch.int32)
+    i32 = torch.int32
+    dev = weights.get_device()
+    if not (weights.dtype is torch.float32 and block_tables.dtype is i32 and
+            ctx_lens.dtype is i32 and weights.is_contiguous() and block_tables.is_contiguous() and
+            ctx_lens.is_contiguous() and dev >= 0 and
+            dev == block_tables.get_device() == ctx_lens.get_device()):
+        _dev(weights, "weights", torch.float32)  # says which and why
+        _dev(block_tables, "block_tables", i32), _dev(ctx_lens, "ctx_lens", i32)
+        _one_device(dev, ((block_tables, "block_tables"), (ctx_lens, "ctx_lens")))
     if weights.dim() not in (3, 4) or block_tables.dim() != 2 or ctx_lens.dim() != 1 or \
             block_tables.shape[0] != ctx_lens.shape[0]:
         raise ValueError("weights [.., num_blocks, Hkv, 16], one table row and length a sequence")
-    _one_device(weights.get_device(), ((block_tables, "block_tables"), (ctx_lens, "ctx_lens"),
-                                       (keep, "keep"), (new_lens, "new_lens")))
+    _one_device(dev, ((keep, "keep"), (new_lens, "new_lens")))
     n_layers = weights.shape[0] if weights.dim() == 4 else 1
     nb, hkv, bs = weights.shape[-3:]
     B, mbs = block_tables.shape
@@ -872,7 +902,7 @@ def evict_select(weights: torch.Tensor, block_tables: torch.Tensor, ctx_lens: to
         new_lens = weights.new_empty(B, dtype=torch.int32)
     elif _dev(new_lens, "new_lens", torch.int32).shape != (B,):
         raise ValueError("new_lens must be [B]")
-    _launch(weights.get_device(), lib().rkv_evict_select, keep.data_ptr(), new_lens.data_ptr(),
+    _launch(dev, lib().rkv_evict_select, keep.data_ptr(), new_lens.data_ptr(),
             weights.data_ptr(), nb * hkv * bs, block_tables.data_ptr(), mbs, ctx_lens.data_ptr(),
             B, n_layers, hkv, bs, nb, budget, sinks, recent,
             mbs * bs if max_context is None else max_context)
@@ -887,16 +917,24 @@ def evict_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, keep: torch.Tensor
     0 .. new_lens[b]-1 of dst_tables (int32 [B, blocks]), with their scales and
     sums.  No destination block may be a source of the call or stand twice; the
     source blocks stay as they are for the caller to free."""
-    _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), _dev(keep, "keep", torch.int32)
-    _dev(new_lens, "new_lens", torch.int32), _dev(src_tables, "src_tables", torch.int32)
-    _dev(dst_tables, "dst_tables", torch.int32)
+    i32 = torch.int32
+    dev = k_pool.get_device()
+    if not (keep.dtype is i32 and new_lens.dtype is i32 and src_tables.dtype is i32 and
+            dst_tables.dtype is i32 and k_pool.is_contiguous() and v_pool.is_contiguous() and
+            keep.is_contiguous() and new_lens.is_contiguous() and src_tables.is_contiguous() and
+            dst_tables.is_contiguous() and dev >= 0 and
+            dev == v_pool.get_device() == keep.get_device() == new_lens.get_device() ==
+            src_tables.get_device() == dst_tables.get_device()):
+        _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), _dev(keep, "keep", i32)  # says which
+        _dev(new_lens, "new_lens", i32), _dev(src_tables, "src_tables", i32)     # and why
+        _dev(dst_tables, "dst_tables", i32)
+        _one_device(dev, ((v_pool, "v_pool"), (keep, "keep"), (new_lens, "new_lens"),
+                          (src_tables, "src_tables"), (dst_tables, "dst_tables")))
     if k_pool.dim() not in (4, 5):
         raise ValueError("pools must be [num_blocks, Hkv, 16, D] or [n_layers, ..]")
     code, ks, vs = _pool_code(k_pool, v_pool, k_scale, v_scale, fmt)
-    _one_device(k_pool.get_device(), ((v_pool, "v_pool"), (keep, "keep"), (new_lens, "new_lens"),
-                                      (src_tables, "src_tables"), (dst_tables, "dst_tables"),
-                                      (k_scale, "k_scale"), (v_scale, "v_scale"),
-                                      (weights, "weights")))
+    if ks is not None or weights is not None:
+        _one_device(dev, ((k_scale, "k_scale"), (v_scale, "v_scale"), (weights, "weights")))
     nb, hkv, bs, d = k_pool.shape[-4:]
     n_layers = k_pool.shape[0] if k_pool.dim() == 5 else 1
     B = new_lens.shape[0]
@@ -907,7 +945,7 @@ def evict_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, keep: torch.Tensor
         raise ValueError("one source and one destination table row per sequence")
     if weights is not None and _dev(weights, "weights", torch.float32).shape != k_pool.shape[:-1]:
         raise ValueError("weights must be the pools' shape without head_dim")
-    _launch(k_pool.get_device(), lib().rkv_evict_compact, k_pool.data_ptr(), v_pool.data_ptr(), ks,
+    _launch(dev, lib().rkv_evict_compact, k_pool.data_ptr(), v_pool.data_ptr(), ks,
             vs, weights.data_ptr() if weights is not None else None, nb * hkv * bs * d,
             nb * hkv * bs, keep.data_ptr(), new_lens.data_ptr(), keep.shape[-1],
             src_tables.data_ptr(), src_tables.shape[1], dst_tables.data_ptr(), dst_tables.shape[1],

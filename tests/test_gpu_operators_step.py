@@ -432,3 +432,23 @@ def test_pools_past_32_bit_offsets(dev, fmt):
     assert results[0][-5].any() and results[0][-3].any()
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_a_smaller_v_pool_is_refused(dev):
+    """The kernels index V by K's shape."""
+    say("smaller v pool")
+    t, freq, _ = small(dev)
+    v8, vs, v = t["v8"][:5].clone(), t["vs"][:5].clone(), t["v"][:5].clone()
+    q8 = (t["k8"], v8, t["ks"], vs)
+    keep = torch.zeros((2, HKV, 4), dtype=torch.int32, device=dev)
+    left = torch.full((2,), 4, dtype=torch.int32, device=dev)
+    for call in (
+            lambda: kv.append_block_q(*q8, t["kn"], t["vn"], t["start"], t["tab"], t["ctx"]),
+            lambda: kv.decode_attention_q(t["q"], *q8, t["tab"], t["ctx"], fmt="int8_block"),
+            lambda: kv.prefill_attention_q(t["q"], *q8, t["tab"], t["start"], t["ctx"]),
+            lambda: kv.gather_q(*q8, t["tab"], t["ctx"], fmt="fp8_block"),
+            lambda: kv.decode_attention_weights(t["q"], t["k"], v, t["w"], t["tab"], t["ctx"]),
+            lambda: kv.evict_compact(t["k"], v, keep, left, t["tab"], t["dst"]),
+            lambda: kv.rope_append(t["q"], t["kn"], t["vn"], t["pos"], freq, t["k"], v, t["slots"])):
+        with pytest.raises(ValueError):
+            call()
