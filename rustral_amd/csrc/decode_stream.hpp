@@ -392,8 +392,12 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
   // significant bits), and in the builds that came with the block-scaled formats
   // and the scores a third (24 bits, as many as fp32: 3.6e-6 off the exact rows
   // with two, about 4e-7 with three).  The operand has 16 rows, so the third term
-  // of up to 5 heads takes rows that were zero; the earlier builds keep their bits.
+  // of up to 5 heads takes rows that were zero; that of 8 heads is an operand of its
+  // own in the rows of the first, a second product onto the same sums (THIRD; 64 x
+  // U[512, 4096], 64 query and 8 KV heads of 128: bf16 with scores 153.4 -> 154.0 us,
+  // int8 with one scale a tile 83.7 -> 87.4).  The earlier builds keep their bits.
   constexpr int TERMS = (TSC || MODE == kScores) && G <= 4 ? 3 : 2;
+  constexpr bool THIRD = (TSC || MODE == kScores) && G > 5;
   static_assert(QNT == (sizeof(T) == 1), "1-byte element type iff a 1-byte format");
   constexpr bool MFMA = (sizeof(T) == 2 || QNT) && 2 * G <= 16;
   // PV on the matrix cores as well (bf16 and 1-byte pools):
@@ -658,6 +662,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
   // MFMA A operands: q split into bf16 hi + lo rows, two values per
   // v_cvt_pk_bf16_f32 (round to nearest even, no branch)
   uint4 qa[MFMA ? NC : 1];
+  uint4 qt[MFMA && THIRD ? NC : 1];  // the third terms, rows 0 .. G - 1
   float qmul = 0.0f;  // I8QK: M_h / 127 of head kq (inf when q_h holds NaN or inf)
   if constexpr (I8QK) {
     // M_h over the 16 lanes of head l / 16 (a NaN counts as inf: the limbs
@@ -712,7 +717,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
   } else if constexpr (MFMA) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      uint32_t h[4];
+      uint32_t h[4], h3[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = qv[c * 8 + 2 * e], y = qv[c * 8 + 2 * e + 1];
@@ -720,13 +725,15 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
         const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xffff0000u);
         const uint32_t lo = cvt_bf16x2(rx, ry);
         h[e] = kt < G ? hi : (kt < 2 * G ? lo : 0u);
-        if constexpr (TERMS == 3) {
+        if constexpr (TERMS == 3 || THIRD) {
           const uint32_t last = cvt_bf16x2(rx - __uint_as_float(lo << 16),
                                            ry - __uint_as_float(lo & 0xffff0000u));
-          h[e] = kt >= 2 * G && kt < 3 * G ? last : h[e];
+          if constexpr (THIRD) h3[e] = kt < G ? last : 0u;
+          else h[e] = kt >= 2 * G && kt < 3 * G ? last : h[e];
         }
       }
       qa[c] = make_uint4(h[0], h[1], h[2], h[3]);
+      if constexpr (THIRD) qt[c] = make_uint4(h3[0], h3[1], h3[2], h3[3]);
     }
   }
 
@@ -816,20 +823,31 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
         } else if constexpr (QNT) {
 #pragma unroll
           for (int n = 0; n < NL; ++n) {
+            const auto k0 = __builtin_bit_cast(bf16x8_t, to_bf16x8_q<FMT>(kb[n].x, kb[n].y));
+            const auto k1 = __builtin_bit_cast(bf16x8_t, to_bf16x8_q<FMT>(kb[n].z, kb[n].w));
+            sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, qa[2 * n]),
+                                                          k0, sacc, 0, 0, 0);
+            if constexpr (THIRD)
+              sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8_t, qt[2 * n]), k0, sacc, 0, 0, 0);
             sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, qa[2 * n]),
-                __builtin_bit_cast(bf16x8_t, to_bf16x8_q<FMT>(kb[n].x, kb[n].y)), sacc, 0, 0, 0);
-            sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8_t, qa[2 * n + 1]),
-                __builtin_bit_cast(bf16x8_t, to_bf16x8_q<FMT>(kb[n].z, kb[n].w)), sacc, 0, 0, 0);
+                __builtin_bit_cast(bf16x8_t, qa[2 * n + 1]), k1, sacc, 0, 0, 0);
+            if constexpr (THIRD)
+              sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8_t, qt[2 * n + 1]), k1, sacc, 0, 0, 0);
           }
         } else {
           static_assert(QNT || NL == NC, "one 16-byte K piece per MFMA");
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+          for (int c = 0; c < NC; ++c) {
             sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, qa[c]),
                                                           __builtin_bit_cast(bf16x8_t, kb[c]),
                                                           sacc, 0, 0, 0);
+            if constexpr (THIRD)
+              sacc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, qt[c]),
+                                                            __builtin_bit_cast(bf16x8_t, kb[c]),
+                                                            sacc, 0, 0, 0);
+          }
         }
         // dot * scale (the reference's order), then the token's K row scale
         float qs = q_scale;
@@ -1023,12 +1041,14 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
         const uint32_t l0 = cvt_bf16x2(rx, ry), l1 = cvt_bf16x2(rz, rw);
         uint2 pb = kt < G ? make_uint2(h0, h1)
                           : (kt < 2 * G ? make_uint2(l0, l1) : make_uint2(0u, 0u));
-        if constexpr (TERMS == 3) {
+        uint2 pt = make_uint2(0u, 0u);  // THIRD: the third terms
+        if constexpr (TERMS == 3 || THIRD) {
           const uint32_t t0 = cvt_bf16x2(rx - __uint_as_float(l0 << 16),
                                          ry - __uint_as_float(l0 & 0xffff0000u));
           const uint32_t t1 = cvt_bf16x2(rz - __uint_as_float(l1 << 16),
                                          rw - __uint_as_float(l1 & 0xffff0000u));
-          if (kt >= 2 * G && kt < 3 * G) pb = make_uint2(t0, t1);
+          if constexpr (THIRD) pt = kt < G ? make_uint2(t0, t1) : pt;
+          else if (kt >= 2 * G && kt < 3 * G) pb = make_uint2(t0, t1);
         }
         // A = V^T: this lane's read address is key 4 kq + (kt >> 2), dims
         // 16 c + 4 (kt & 3) .. + 3
@@ -1038,6 +1058,9 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
           const uint2 a = lds_read_tr16(va + 32 * c);
           ov[c] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
               __builtin_bit_cast(bf16x4_t, a), __builtin_bit_cast(bf16x4_t, pb), ov[c], 0, 0, 0);
+          if constexpr (THIRD)
+            ov[c] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+                __builtin_bit_cast(bf16x4_t, a), __builtin_bit_cast(bf16x4_t, pt), ov[c], 0, 0, 0);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // reads done before the
         __builtin_amdgcn_wave_barrier();                         // next tile overwrites
@@ -1075,7 +1098,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
         const float4 p0 = reinterpret_cast<const float4*>(pp)[0];
         const float4 p1 = reinterpret_cast<const float4*>(pp)[1];
         const float pv8[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-        uint32_t pw[4];
+        uint32_t pw[4], pt[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = pv8[2 * e], y = pv8[2 * e + 1];
@@ -1084,10 +1107,11 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
           const float ry = y - __uint_as_float(hi & 0xffff0000u);
           const uint32_t lo = cvt_bf16x2(rx, ry);
           pw[e] = kt < G ? hi : (kt < 2 * G ? lo : 0u);
-          if constexpr (TERMS == 3) {
+          if constexpr (TERMS == 3 || THIRD) {
             const uint32_t last = cvt_bf16x2(rx - __uint_as_float(lo << 16),
                                              ry - __uint_as_float(lo & 0xffff0000u));
-            pw[e] = kt >= 2 * G && kt < 3 * G ? last : pw[e];
+            if constexpr (THIRD) pt[e] = kt < G ? last : 0u;
+            else pw[e] = kt >= 2 * G && kt < 3 * G ? last : pw[e];
           }
         }
         const uint4 pb = make_uint4(pw[0], pw[1], pw[2], pw[3]);
@@ -1097,9 +1121,13 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd<G, FORMAT, MODE>()))) void dec
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           const uint2 raw = lds_read_tr8(va + 16 * c);
-          ov[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8_t, to_bf16x8_q<FMT>(raw.x, raw.y)),
-              __builtin_bit_cast(bf16x8_t, pb), ov[c], 0, 0, 0);
+          const auto va8 = __builtin_bit_cast(bf16x8_t, to_bf16x8_q<FMT>(raw.x, raw.y));
+          ov[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va8, __builtin_bit_cast(bf16x8_t, pb),
+                                                          ov[c], 0, 0, 0);
+          if constexpr (THIRD)
+            ov[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                va8, __builtin_bit_cast(bf16x8_t, make_uint4(pt[0], pt[1], pt[2], pt[3])), ov[c], 0,
+                0, 0);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // reads done before the
         __builtin_amdgcn_wave_barrier();                         // next pair overwrites

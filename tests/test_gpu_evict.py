@@ -323,3 +323,34 @@ def test_what_no_table_names_is_not_seen(dev, kind, hq, hkv, d):
         got = kv.prefill_attention_q(to_dev(qq, dev), *args, to_dev(start, dev), gc, None, fmt)
         want, bound, _, _ = R.attend(qq, fk, fv, tables, ctx, 1 / math.sqrt(d), n, start)
         R.assert_within(to_np(got), want, bound, "prefill")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8", "fp8", "int8_block", "fp8_block"])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (16, 4, 64), (4, 2, 128), (2, 2, 64)])
+def test_precision_of_the_products(dev, kind, hq, hkv, d):
+    """Queries and weights enter the matrix cores with 24 bits at every group size.  What is
+    left are the roundings of some 128 fp32 additions of partial sums of about 1: 11 steps
+    of 2^-25 when they are independent, 3.4e-7; 2^-20 is three times that, and two bf16
+    terms (2^-17 of each of 128 products, as many independent) would be 3e-6 off."""
+    say(f"precision {kind} hq={hq} hkv={hkv} d={d}")
+    rng = np.random.default_rng(5)
+    ctx = np.array([400, 1300], np.int32)
+    nb = 110
+    tables = make_tables(rng, ctx, 16, nb)
+    (k, v, ks, vs), (fk, fv) = pools_of(rng, nb, hkv, d, kind)
+    q = rng.standard_normal((2, hq, d)).astype(np.float32)
+    want, _, ws, _ = R.attend(q, fk, fv, tables, ctx, 1 / math.sqrt(d))
+    fmt = kind if kind != "bf16" else None
+    scales = dict(k_scale=to_dev(ks, dev), v_scale=to_dev(vs, dev)) if fmt else {}
+    w = torch.zeros((nb, hkv, 16), device=dev)
+    gk, gv, gt, gc = (to_dev(a, dev) for a in (k, v, tables, ctx))
+    outs = [kv.decode_attention_weights(to_dev(q, dev), gk, gv, w, gt, gc, fmt=fmt, **scales)]
+    if kind.endswith("block"):
+        outs.append(kv.decode_attention_q(to_dev(q, dev), gk, gv, *scales.values(), gt, gc, fmt=fmt))
+    for o in outs:
+        assert np.linalg.norm(to_np(o) - want) <= 2.0 ** -20 * np.linalg.norm(want)
+    w = to_np(w)
+    for b in range(2):
+        p = np.arange(ctx[b])
+        got = w[tables[b, p // 16], :, p % 16].T
+        assert np.linalg.norm(got - ws[b]) <= 2.0 ** -20 * np.linalg.norm(ws[b])
