@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import oracle
-from rustral_amd import kv
+from rustral_amd import _lib, kv
 from tests import op_refs as R
 from tests.gpu_util import say, to_dev, to_np
 from tests.helpers import contexts, make_tables
@@ -354,3 +354,53 @@ def test_precision_of_the_products(dev, kind, hq, hkv, d):
         p = np.arange(ctx[b])
         got = w[tables[b, p // 16], :, p % 16].T
         assert np.linalg.norm(got - ws[b]) <= 2.0 ** -20 * np.linalg.norm(ws[b])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,lo,hi", [(4, 4, 1, 90), (8, 4, 100, 600), (8, 1, 700, 2100)])
+def test_weights_of_narrow_heads(dev, kind, hq, hkv, lo, hi):
+    say(f"weights d=32 {kind} hq={hq} hkv={hkv}")
+    rng = np.random.default_rng(hi)
+    ctx = contexts(rng, 3, lo, hi)
+    nb = int(((ctx + 15) // 16).sum()) + 1
+    tables = make_tables(rng, ctx, 16, nb)
+    (k, v, _, _), (fk, fv) = pools_of(rng, nb, hkv, 32, kind)
+    q = rng.standard_normal((3, hq, 32)).astype(np.float32)
+    want, bound, ws, wb = R.attend(q, fk, fv, tables, ctx, 1 / math.sqrt(32))
+    w = torch.zeros((nb, hkv, 16), device=dev)
+    out = kv.decode_attention_weights(to_dev(q, dev), to_dev(k, dev), to_dev(v, dev), w,
+                                      to_dev(tables, dev), to_dev(ctx, dev))
+    R.assert_within(to_np(out), want, bound, "attention")
+    w = to_np(w)
+    for b in range(3):
+        p = np.arange(ctx[b])
+        R.assert_within(w[tables[b, p // 16], :, p % 16].T, ws[b], wb[b] + 2.0 ** -23 * ws[b], "sums")
+
+
+def test_shapes_without_a_kernel_are_refused(dev):
+    say("no kernel")
+    z = lambda *s, t=torch.float32: torch.zeros(s, dtype=t, device=dev)
+    tab, ctx = z(1, 2, t=torch.int32), torch.full((1,), 5, dtype=torch.int32, device=dev)
+    w = z(4, 2, 16)
+    for hq, d, fmt in ((6, 64, None), (32, 64, None), (2, 48, None), (2, 32, "int8_block"),
+                       (6, 64, "fp8_block"), (2, 32, "int8")):
+        t = torch.float32 if fmt is None else torch.uint8
+        k, v = z(4, 2, 16, d, t=t), z(4, 2, 16, d, t=t)
+        s = {}
+        if fmt:
+            shape = (4, 2) if fmt.endswith("block") else (4, 2, 16)
+            s = dict(k_scale=z(*shape), v_scale=z(*shape), fmt=fmt)
+        with pytest.raises(_lib.RkvError):
+            kv.decode_attention_weights(z(1, hq, d), k, v, w, tab, ctx, **s)
+        if fmt and fmt.endswith("block"):
+            with pytest.raises(_lib.RkvError):
+                kv.decode_attention_q(z(1, hq, d), k, v, s["k_scale"], s["v_scale"], tab, ctx,
+                                      fmt=fmt)
+            with pytest.raises(_lib.RkvError):
+                kv.prefill_attention_q(z(1, hq, d), k, v, s["k_scale"], s["v_scale"], tab,
+                                       torch.tensor([0, 1], dtype=torch.int32, device=dev), ctx,
+                                       fmt=fmt)
+    with pytest.raises(ValueError):      # the fused append takes row-scaled pools
+        kv.decode_attention_append_q(z(1, 2, 64), z(4, 2, 16, 64, t=torch.uint8),
+                                     z(4, 2, 16, 64, t=torch.uint8), z(4, 2), z(4, 2), z(1, 2, 64),
+                                     z(1, 2, 64), tab, ctx, fmt="int8_block")
