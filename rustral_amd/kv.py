@@ -482,11 +482,11 @@ def decode_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     code = _anycode(fmt)
     u8, f32, i32 = torch.uint8, torch.float32, torch.int32
     dev = q.get_device()
-    if not (q.dtype is f32 and k_pool.dtype is u8 and v_pool.dtype is u8 and
+    if not (dev >= 0 and q.dtype is f32 and k_pool.dtype is u8 and v_pool.dtype is u8 and
             k_scale.dtype is f32 and v_scale.dtype is f32 and block_tables.dtype is i32 and
             ctx_lens.dtype is i32 and q.is_contiguous() and k_pool.is_contiguous() and
             v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous() and
-            block_tables.is_contiguous() and ctx_lens.is_contiguous() and dev >= 0 and
+            block_tables.is_contiguous() and ctx_lens.is_contiguous() and
             dev == k_pool.get_device() == v_pool.get_device() == k_scale.get_device() ==
             v_scale.get_device() == block_tables.get_device() == ctx_lens.get_device()):
         _dev(q, "q", f32), _dev(k_pool, "k_pool", u8)  # says which and why
@@ -571,13 +571,13 @@ def append_block_q(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Te
     code = _bcode(fmt)
     u8, f32, i32 = torch.uint8, torch.float32, torch.int32
     dev = k_pool.get_device()
-    if not (k_pool.dtype is u8 and v_pool.dtype is u8 and k_scale.dtype is f32 and
+    if not (dev >= 0 and k_pool.dtype is u8 and v_pool.dtype is u8 and k_scale.dtype is f32 and
             v_scale.dtype is f32 and k_new.dtype is f32 and v_new.dtype is f32 and
             new_start.dtype is i32 and block_tables.dtype is i32 and ctx_lens.dtype is i32 and
             k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and
             v_scale.is_contiguous() and k_new.is_contiguous() and v_new.is_contiguous() and
             new_start.is_contiguous() and block_tables.is_contiguous() and
-            ctx_lens.is_contiguous() and dev >= 0 and
+            ctx_lens.is_contiguous() and
             dev == v_pool.get_device() == k_scale.get_device() == v_scale.get_device() ==
             k_new.get_device() == v_new.get_device() == new_start.get_device() ==
             block_tables.get_device() == ctx_lens.get_device()):
@@ -624,12 +624,12 @@ def prefill_attention_q(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
     code = _bcode(fmt)
     u8, f32, i32 = torch.uint8, torch.float32, torch.int32
     dev = q.get_device()
-    if not (q.dtype is f32 and k_pool.dtype is u8 and v_pool.dtype is u8 and
+    if not (dev >= 0 and q.dtype is f32 and k_pool.dtype is u8 and v_pool.dtype is u8 and
             k_scale.dtype is f32 and v_scale.dtype is f32 and block_tables.dtype is i32 and
             q_start.dtype is i32 and ctx_lens.dtype is i32 and q.is_contiguous() and
             k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and
             v_scale.is_contiguous() and block_tables.is_contiguous() and
-            q_start.is_contiguous() and ctx_lens.is_contiguous() and dev >= 0 and
+            q_start.is_contiguous() and ctx_lens.is_contiguous() and
             dev == k_pool.get_device() == v_pool.get_device() == k_scale.get_device() ==
             v_scale.get_device() == block_tables.get_device() == q_start.get_device() ==
             ctx_lens.get_device()):
@@ -739,12 +739,12 @@ def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     f32 = torch.float32
     dev = q.get_device()
     qs, ns, vs_ = q.stride(), k_new.stride(), v_new.stride()
-    if not (q.dtype is f32 and k_new.dtype is f32 and v_new.dtype is f32 and
+    if not (dev >= 0 and q.dtype is f32 and k_new.dtype is f32 and v_new.dtype is f32 and
             positions.dtype is torch.int32 and inv_freq.dtype is torch.float64 and
             slot_mapping.dtype is torch.int64 and qs[-1] == 1 and ns[-1] == 1 and
             vs_[-1] == 1 and positions.is_contiguous() and inv_freq.is_contiguous() and
             slot_mapping.is_contiguous() and k_pool.is_contiguous() and
-            v_pool.is_contiguous() and dev >= 0 and
+            v_pool.is_contiguous() and
             dev == k_new.get_device() == v_new.get_device() == positions.get_device() ==
             inv_freq.get_device() == k_pool.get_device() == v_pool.get_device() ==
             slot_mapping.get_device()):
@@ -828,10 +828,10 @@ def decode_attention_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
     pools.  workspace: weights_workspace_bytes."""
     f32, i32 = torch.float32, torch.int32
     dev = q.get_device()
-    if not (q.dtype is f32 and weights.dtype is f32 and block_tables.dtype is i32 and
+    if not (dev >= 0 and q.dtype is f32 and weights.dtype is f32 and block_tables.dtype is i32 and
             ctx_lens.dtype is i32 and q.is_contiguous() and weights.is_contiguous() and
             k_pool.is_contiguous() and v_pool.is_contiguous() and
-            block_tables.is_contiguous() and ctx_lens.is_contiguous() and dev >= 0 and
+            block_tables.is_contiguous() and ctx_lens.is_contiguous() and
             dev == k_pool.get_device() == v_pool.get_device() == weights.get_device() ==
             block_tables.get_device() == ctx_lens.get_device()):
         _dev(q, "q", f32), _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool")  # says which and why
@@ -879,9 +879,9 @@ def evict_select(weights: torch.Tensor, block_tables: torch.Tensor, ctx_lens: to
     new_lens int32 [B])."""
     i32 = torch.int32
     dev = weights.get_device()
-    if not (weights.dtype is torch.float32 and block_tables.dtype is i32 and
+    if not (dev >= 0 and weights.dtype is torch.float32 and block_tables.dtype is i32 and
             ctx_lens.dtype is i32 and weights.is_contiguous() and block_tables.is_contiguous() and
-            ctx_lens.is_contiguous() and dev >= 0 and
+            ctx_lens.is_contiguous() and
             dev == block_tables.get_device() == ctx_lens.get_device()):
         _dev(weights, "weights", torch.float32)  # says which and why
         _dev(block_tables, "block_tables", i32), _dev(ctx_lens, "ctx_lens", i32)
@@ -919,10 +919,10 @@ def evict_compact(k_pool: torch.Tensor, v_pool: torch.Tensor, keep: torch.Tensor
     source blocks stay as they are for the caller to free."""
     i32 = torch.int32
     dev = k_pool.get_device()
-    if not (keep.dtype is i32 and new_lens.dtype is i32 and src_tables.dtype is i32 and
+    if not (dev >= 0 and keep.dtype is i32 and new_lens.dtype is i32 and src_tables.dtype is i32 and
             dst_tables.dtype is i32 and k_pool.is_contiguous() and v_pool.is_contiguous() and
             keep.is_contiguous() and new_lens.is_contiguous() and src_tables.is_contiguous() and
-            dst_tables.is_contiguous() and dev >= 0 and
+            dst_tables.is_contiguous() and
             dev == v_pool.get_device() == keep.get_device() == new_lens.get_device() ==
             src_tables.get_device() == dst_tables.get_device()):
         _dev(k_pool, "k_pool"), _dev(v_pool, "v_pool"), _dev(keep, "keep", i32)  # says which
