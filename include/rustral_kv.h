@@ -419,7 +419,8 @@ int rkv_rope_frequencies(double* inv_freq, float* magnitude, int rotary_dim, dou
  * of what its memory held.  max_new: host-side bound on the n_b (it sizes the
  * grid); only the first max_new rows of a sequence are written.  Negative
  * positions, positions past the table and block ids outside the pool are
- * skipped.  A block must not be appended to through two sequences of the call.
+ * skipped.  A block must not be appended to through two entries of the tables in one
+ * call (its scale would have two writers).
  * Strides as rkv_append; pool_layer_stride in bytes, the scale pools' is
  * pool_layer_stride / (16 * head_dim).  block_size 16; head_dim 32, 64 or 128. */
 int rkv_append_block_q(void* k_pool, void* v_pool, float* k_scale, float* v_scale,

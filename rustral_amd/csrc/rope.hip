@@ -273,15 +273,15 @@ __global__ __launch_bounds__(256) void rope_append_kernel(
 }
 
 int check_rope(const char* who, int64_t n_tokens, int num_heads, int head_dim, int rotary_dim) {
-  const std::string w = std::string(who) + ": ";
+  const auto bad = [&](int rc, const char* what) { return fail(rc, std::string(who) + what); };
   if (n_tokens < 0 || num_heads <= 0)
-    return fail(RKV_ERR_INVALID_ARG, w + "n_tokens must be >= 0 and the head counts > 0");
+    return bad(RKV_ERR_INVALID_ARG, ": n_tokens must be >= 0 and the head counts > 0");
   if (n_tokens > 0x7fffffff)
-    return fail(RKV_ERR_INVALID_ARG, w + "n_tokens too large for one launch");
+    return bad(RKV_ERR_INVALID_ARG, ": n_tokens too large for one launch");
   if (head_dim <= 0 || head_dim % 8 || head_dim > 1024)
-    return fail(RKV_ERR_UNSUPPORTED, w + "head_dim must be a multiple of 8 up to 1024");
+    return bad(RKV_ERR_UNSUPPORTED, ": head_dim must be a multiple of 8 up to 1024");
   if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > head_dim)
-    return fail(RKV_ERR_INVALID_ARG, w + "rotary_dim must be even, > 0 and <= head_dim");
+    return bad(RKV_ERR_INVALID_ARG, ": rotary_dim must be even, > 0 and <= head_dim");
   return RKV_OK;
 }
 

@@ -184,3 +184,26 @@ def test_rope_front_end_refuses(dev):
     with pytest.raises(ValueError):
         kv.rope_append(x, x, x, pos, f, p.to(torch.uint8), p.to(torch.uint8), slots, fmt="int8")
     assert kv.rope(x[:0], pos[:0], f).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("d,rot", [(8, 8), (24, 24), (40, 18), (1024, 1024), (128, 2)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_negative_positions_and_odd_widths(dev, d, rot, interleaved):
+    """Positions down to -2^31, every head width the call takes; a turn there and back."""
+    say(f"rope negative d={d} rot={rot} interleaved={interleaved}")
+    rng = np.random.default_rng(d)
+    pos = np.array([-1, 0, -2 ** 31, 2 ** 31 - 1, -77777, 5], np.int32)
+    f, _ = kv.rope_frequencies(rot, device=dev)
+    x = rng.standard_normal((len(pos), 3, d)).astype(np.float32)
+    y = kv.rope(to_dev(x, dev), to_dev(pos, dev), f, interleaved=interleaved)
+    freq = f.cpu().numpy()
+    R.assert_within(to_np(y), R.rope(x, pos, freq, interleaved),
+                    R.rope_bound(x, pos, freq, interleaved), "negative")
+    some = pos[[0, 1, 4, 5]]
+    back = to_np(kv.rope(y[[0, 1, 4, 5]].contiguous(), to_dev(-some, dev), f,
+                         interleaved=interleaved))
+    x = x[[0, 1, 4, 5]]
+    # the first turn's errors on a pair reach each element (2 bounds), and the second's
+    # own is that of a pair sqrt(2) as large at most
+    R.assert_within(back, x.astype(np.float64), 3.5 * R.rope_bound(x, some, freq, interleaved),
+                    "there and back")
