@@ -12,6 +12,8 @@
 // 512 7.6 / 22.3 (with the mask and the history requested only after the first barrier
 // 7.8 / 22.8); 2,048 with 256 7.4 / 23.2; 8,192 with 1,024 8.4 / 23.1.  With streaming
 // stores 7.7 / 21.3; streaming loads as well 22.9 (a caller's logits are often cached).
+// One workgroup of 1,024 threads for a whole row (no second launch): 1 x 5,000 6.9 for
+// 7.6, 1 x 16,384 9.7 for 7.7, 1 x 32,000 15.0 for 7.7: not for a vocabulary's length.
 #include "../../include/rustral_model.h"
 #include "common.hpp"
 

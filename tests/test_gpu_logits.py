@@ -1,4 +1,6 @@
 """process_logits on the GPU against the formulas in 64 bits."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -149,3 +151,24 @@ def test_front_end_refuses(dev):
         model.process_logits(x, bias_ids=i)
     got, pick = model.process_logits(x[:0])
     assert got.shape == (0, 100) and pick.shape == (0,)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 257])
+@pytest.mark.parametrize("n", [4097, 16381, 16384, 16385, 32000, 32767, 32768, 32769])
+def test_borders_of_slices_and_rows(dev, rows, n):
+    """Lengths on both sides of multiples of a slice, for few rows and for more than the
+    chip has CUs; rows on and off a 16-byte boundary give the same bits."""
+    say(f"logits rows={rows} n={n}")
+    rng = np.random.default_rng(rows + n)
+    x, a = make(rng, rows, n, 300, 5, 1)
+    got, pick = call(dev, x, a)
+    wide = torch.zeros((rows, n + 5), device=dev)
+    wide[:, 1:n + 1] = to_dev(x, dev)
+    off, off_pick = call(dev, wide[:, 1:n + 1], a)
+    assert torch.equal(got.view(torch.int32), off.view(torch.int32)) and torch.equal(pick, off_pick)
+    some = min(rows, 3)                       # the formulas on the first rows
+    b = {k: v[:some] if len(v) == rows else v for k, v in a.items()}
+    b["start"], b["bias_start"] = a["start"][:some + 1], a["bias_start"][:some + 1]
+    check(got[:some], pick[:some], x[:some], b)
+    best = torch.where(got.isnan(), -math.inf, got).max(1).values
+    assert torch.equal(got.gather(1, pick.long()[:, None])[:, 0], best)
